@@ -598,6 +598,136 @@ int b200q_gather_elements_dev(const void *src, int32_t elem_bytes, const void *i
 int b200q_top_fake_quant_f32_dev(const float *x, float *y, int64_t count, double threshold, void *stream);
 int b200q_top_distance_f32_dev(const float *x, const float *ref, int64_t count, double *sums5, void *stream);
 
+/* ------------------------------------------------------------------ decoding over a paged key / value cache
+ * What a decoder needs between its A16MatMul projections: rotary positions, a cache of keys and values in pages, attention
+ * over it for one token or a tree of drafted tokens, and the pages' bookkeeping.  (The reference lowers these to TPU codegen
+ * ops without an inference body in its interpreter; no counterpart there.)  Device face only: every pointer inside the
+ * structs is a DEVICE pointer of one device, the structs themselves are read during the call; calls are asynchronous on
+ * `stream`, allocate nothing and never synchronise, so they can be captured.  They run on the device that holds the pool's
+ * tables (or x), whichever device is current.  `stream` belongs to that device, or is NULL for its legacy default stream.
+ * What only the device sees (lengths, page numbers, row starts, paths) is never trusted with an address: a page number
+ * outside the pool or a position past the table is not read or written, as each function says. */
+
+/* Keys and values: element (layer, page, slot, head, d) of either lies at layer * layer_stride + page * page_stride +
+ * slot * slot_stride + head * head_stride + d, in elements; any order of the dimensions.  k, v 16-byte aligned, strides
+ * multiples of 8 elements, head_dim a multiple of 8 up to 256, dtype B200Q_DT_BF16 or B200Q_DT_F16.  The number of pages and
+ * of slots in a page stand in the pool. */
+typedef struct {
+  void *k, *v;
+  int64_t layer_stride, page_stride, slot_stride, head_stride;
+  int32_t layers, heads, head_dim, dtype;
+} b200q_kv_cache;
+
+/* Which pages a sequence holds.  Position p of sequence s lies in page table[s * table_stride + p / page_size], slot
+ * p % page_size, for p / page_size < table_width; entries past held[s] are not meaningful (-1 where a call here cleared
+ * them).  length[s] positions are committed; refcount[p] sequences hold page p, 0 means free.  A new pool is refcount = 0,
+ * held = 0, length = 0.  `scratch` is working space of at least b200q_kv_scratch_words(sequences) words whose contents need not be
+ * kept: calls that use it (fork, compact) and can overlap need pools with scratch of their own.  Limits: 1024 sequences,
+ * 1048576 pages, table_width * page_size below 2^31. */
+typedef struct {
+  int32_t *table, *length, *held, *refcount, *scratch;
+  int64_t table_stride;
+  int32_t sequences, table_width, pages, page_size;
+  int64_t scratch_words;
+} b200q_kv_pool;
+int64_t b200q_kv_scratch_words(int32_t sequences);
+
+/* Every sequence s with extra[s] >= 0 afterwards holds the pages of at least length[s] + extra[s] positions: the
+ * lowest-numbered free pages, in the order of the sequences and of their positions.  All or nothing: when the free pages do
+ * not suffice, or a row of the table would, nothing changes and *status (optional) becomes 1 or 2; it is left alone
+ * otherwise. */
+int b200q_kv_reserve_dev(const b200q_kv_pool *pool, const int32_t *extra, int32_t *status, void *stream);
+/* Every sequence with which[s] != 0 gives its pages back (a page is free when its last holder has) and is empty afterwards. */
+int b200q_kv_free_dev(const b200q_kv_pool *pool, const int32_t *which, void *stream);
+/* Every sequence s with a parent[s] other than s in [0, sequences) becomes what that sequence was BEFORE the call (beams
+ * reordered in one call; swaps and several children of one parent included); other values of parent leave s alone.  Full
+ * pages are shared; the filled slots of a ragged last page are copied in every layer into a page of the child's own (the
+ * lowest-numbered pages free before the call, in the order of the sequences); pages held past the parent's length are not passed on;
+ * what s held is given back after that.  When the free pages do not suffice nothing changes and *status (optional) becomes 1. */
+int b200q_kv_fork_dev(const b200q_kv_cache *cache, const b200q_kv_pool *pool, const int32_t *parent, int32_t *status, void *stream);
+/* Keeps the accepted path of a tree of drafted tokens whose entries stand at positions length[s] + node: for i below
+ * path_length[s], in order, the entry of node path[s * path_stride + i] moves to position length[s] + i in every layer, and
+ * length_out[s] = length[s] + the number of nodes moved.  Nodes of a path ascend strictly (a parent comes before its
+ * children); the path ends before the first entry that does not, or whose page or destination is not in the pool.
+ * length_out may be the pool's length, and must not overlap it otherwise.  path_width <= 1024 entries a row. */
+int b200q_kv_compact_dev(const b200q_kv_cache *cache, const b200q_kv_pool *pool, const int32_t *path, int64_t path_stride,
+                         int32_t path_width, const int32_t *path_length, int32_t *length_out, void *stream);
+
+/* Rotary positions.  Pair i of the first rotary_dim elements of a head is (x[2i], x[2i+1]) when interleaved, else
+ * (x[i], x[i + rotary_dim / 2]); it is turned by the angle position * frequency[i] and multiplied by magnitude.  Elements
+ * from rotary_dim on pass through.  Angles are formed and reduced in 64 bits, products in 32, the result is rounded once. */
+typedef enum {
+  B200Q_ROPE_SCALING_NONE = 0,      /* f_i = base^(-2i / rotary_dim) */
+  B200Q_ROPE_SCALING_LINEAR = 1,    /* f_i / factor */
+  B200Q_ROPE_SCALING_STRETCHED = 2, /* base * factor^(r / (r - 2)) in place of base (r = rotary_dim > 2) */
+  B200Q_ROPE_SCALING_YARN = 3,      /* from f_i (pairs that turn high_turns times or more over original_positions) to
+                                     * f_i / factor (low_turns or fewer), linear in the pair's index between; the magnitude is
+                                     * 0.1 ln(factor) + 1 */
+  B200Q_ROPE_SCALING_BANDED = 4     /* the same two ends, linear in the number of turns between; magnitude 1 */
+} b200q_rope_scaling_kind;
+typedef struct {
+  int32_t kind;
+  double factor;             /* >= 1 */
+  double original_positions; /* YARN, BANDED: the positions that the model was trained on */
+  double low_turns, high_turns;
+} b200q_rope_scaling;
+typedef struct {
+  int32_t head_dim, rotary_dim, interleaved;
+  float magnitude;
+  double frequency[128]; /* radians per position */
+} b200q_rope_plan;
+/* Fills a plan (host code, no device needed).  rotary_dim even, at most head_dim <= 256; scaling NULL = none.  A program with
+ * frequencies of its own writes them into the plan. */
+int b200q_rope_plan_init(b200q_rope_plan *plan, int32_t head_dim, int32_t rotary_dim, int32_t interleaved, double base,
+                         const b200q_rope_scaling *scaling);
+/* y = rotated x: 16-bit x [rows][heads][head_dim] with strides in elements, positions [rows] int32.  y may be x (the same strides), and
+ * must not overlap it otherwise. */
+int b200q_rope_dev(const b200q_rope_plan *plan, const void *x, void *y, const int32_t *positions, int64_t rows, int32_t heads,
+                   int64_t x_row_stride, int64_t x_head_stride, int64_t y_row_stride, int64_t y_head_stride, int32_t dtype,
+                   void *stream);
+/* One layer's new rows: row r of sequence s (row_start[s] <= r < row_start[s + 1]) is its node n = r - row_start[s] and
+ * belongs at position length[s] + n.  q is rotated into q_out; k is rotated and v copied into the cache there.  positions [rows]
+ * names the angles' positions (a tree's depths), NULL = where the rows belong.  Rows outside every sequence stay as they are, and a
+ * row whose position has no page is rotated but not written.  k and v have the cache's heads; q may be q_out. */
+typedef struct {
+  const void *q;
+  void *q_out;
+  const void *k, *v;
+  const int32_t *row_start;  /* [sequences + 1], ascending */
+  const int32_t *positions;
+  int64_t q_row_stride, q_head_stride, q_out_row_stride, q_out_head_stride, k_row_stride, k_head_stride, v_row_stride, v_head_stride;
+  int64_t rows;
+  int32_t q_heads, layer;
+} b200q_rope_append;
+int b200q_rope_append_dev(const b200q_rope_plan *plan, const b200q_kv_cache *cache, const b200q_kv_pool *pool,
+                          const b200q_rope_append *args, void *stream);
+
+/* Attention of the rows that were appended: row r = node n of sequence s, head h attends, in cache head
+ * h / (q_heads / heads), to the committed positions [0, length[s]) and to the drafted nodes m of s (position length[s] + m)
+ * that its mask names: bit m % 32 of mask[r * mask_stride + m / 32], words past mask_stride counting as 0.  mask NULL: a
+ * chain, m <= n (one row a sequence: plain decoding).
+ *   out = sum_j w_j v_j / sum_j w_j,  w_j = exp(scale * (q . k_j) - max)
+ * A row that sees nothing (and one whose scores are all -inf) becomes zeros; what a row does not see does not touch it, infinities
+ * and NaN included.  Positions whose page is not in the pool are not seen.  Rows outside every sequence stay as they are.  Products and sums in
+ * fp32, the weights rounded to the 16-bit type before the second product.  q, out 16-byte aligned with strides of multiples of 8
+ * elements; scale positive.  workspace: b200q_tree_attention_workspace bytes, 16-byte aligned, contents irrelevant before and after;
+ * calls that can overlap (two captured graphs replayed at a time among them) need one each. */
+typedef struct {
+  const void *q;
+  void *out;
+  const int32_t *row_start;  /* [sequences + 1], ascending */
+  const uint32_t *mask;
+  void *workspace;
+  int64_t workspace_bytes;
+  int64_t q_row_stride, q_head_stride, out_row_stride, out_head_stride, mask_stride;
+  int64_t rows;
+  int32_t q_heads, layer;
+  float scale;
+} b200q_tree_attention;
+/* The workspace's size for this cache's head size on the device that holds the cache. */
+int b200q_tree_attention_workspace(const b200q_kv_cache *cache, int32_t q_heads, int64_t *bytes);
+int b200q_tree_attention_dev(const b200q_kv_cache *cache, const b200q_kv_pool *pool, const b200q_tree_attention *args, void *stream);
+
 /* The two symbols of the reference's calibration_math.so (bindings/kld/calibration_math.cpp:326-337), with
  * HOST buffers, so python/calibration/kld_calibrator.py:50-59 can load this library in its place.
  * Failure is reported as NaN (see b200q_last_error). */

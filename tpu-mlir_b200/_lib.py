@@ -18,6 +18,7 @@ RQ_NONE, RQ_MULTIPLIER_SHIFT, RQ_QDM, RQ_MULTIPLIER_SHIFT_F32, RQ_ONLY_SHIFT, RQ
 RELU_NONE, RELU_BEFORE_REQUANT, RELU_AFTER_REQUANT = range(3)
 ALGO_AUTO, ALGO_TENSOR_CORE, ALGO_CUDA_CORE = 0, 1, 2
 LAYOUT_NCHW, LAYOUT_NHWC = 0, 1
+ROPE_SCALING_NONE, ROPE_SCALING_LINEAR, ROPE_SCALING_STRETCHED, ROPE_SCALING_YARN, ROPE_SCALING_BANDED = range(5)
 
 
 class B200QError(RuntimeError):
@@ -86,6 +87,43 @@ class A16MatMulDesc(C.Structure):
     _fields_ = [("M", C.c_int64), ("K", C.c_int64), ("N", C.c_int64), ("weight_bits", C.c_int32),
                 ("q_group_size", C.c_int32), ("w_transpose", C.c_int32), ("with_bias", C.c_int32),
                 ("out_dtype", C.c_int32), ("weight_version", C.c_int32)]
+
+
+class KvCache(C.Structure):
+    """b200q_kv_cache: keys and values in pages, strides in elements."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p)] + \
+               [(n, C.c_int64) for n in ("layer_stride", "page_stride", "slot_stride", "head_stride")] + \
+               [(n, C.c_int32) for n in ("layers", "heads", "head_dim", "dtype")]
+
+
+class KvPool(C.Structure):
+    """b200q_kv_pool: which pages a sequence holds."""
+    _fields_ = [(n, C.c_void_p) for n in ("table", "length", "held", "refcount", "scratch")] + [("table_stride", C.c_int64)] + \
+               [(n, C.c_int32) for n in ("sequences", "table_width", "pages", "page_size")] + [("scratch_words", C.c_int64)]
+
+
+class RopeScaling(C.Structure):
+    _fields_ = [("kind", C.c_int32)] + [(n, C.c_double) for n in ("factor", "original_positions", "low_turns", "high_turns")]
+
+
+class RopePlan(C.Structure):
+    _fields_ = [("head_dim", C.c_int32), ("rotary_dim", C.c_int32), ("interleaved", C.c_int32), ("magnitude", C.c_float),
+                ("frequency", C.c_double * 128)]
+
+
+class RopeAppend(C.Structure):
+    """b200q_rope_append: one layer's new queries, keys and values."""
+    _fields_ = [(n, C.c_void_p) for n in ("q", "q_out", "k", "v", "row_start", "positions")] + \
+               [(n, C.c_int64) for n in ("q_row_stride", "q_head_stride", "q_out_row_stride", "q_out_head_stride", "k_row_stride",
+                                         "k_head_stride", "v_row_stride", "v_head_stride", "rows")] + \
+               [("q_heads", C.c_int32), ("layer", C.c_int32)]
+
+
+class TreeAttention(C.Structure):
+    """b200q_tree_attention: the rows that attend and their masks."""
+    _fields_ = [(n, C.c_void_p) for n in ("q", "out", "row_start", "mask", "workspace")] + [("workspace_bytes", C.c_int64)] + \
+               [(n, C.c_int64) for n in ("q_row_stride", "q_head_stride", "out_row_stride", "out_head_stride", "mask_stride", "rows")] + \
+               [("q_heads", C.c_int32), ("layer", C.c_int32), ("scale", C.c_float)]
 
 
 _FLOATPP = C.POINTER(C.POINTER(C.c_float))
@@ -197,6 +235,17 @@ SIGNATURES = {
     "b200q_calib_find_thresholds": (C.c_int, [C.c_void_p, C.c_int32, C.POINTER(C.c_void_p), C.POINTER(C.c_int64),
                                               C.POINTER(C.c_float), C.c_int64, C.POINTER(C.c_float),
                                               C.POINTER(C.c_float), C.c_void_p]),
+    "b200q_kv_scratch_words": (C.c_int64, [C.c_int32]),
+    "b200q_kv_reserve_dev": (C.c_int, [C.POINTER(KvPool), C.c_void_p, C.c_void_p, C.c_void_p]),
+    "b200q_kv_free_dev": (C.c_int, [C.POINTER(KvPool), C.c_void_p, C.c_void_p]),
+    "b200q_kv_fork_dev": (C.c_int, [C.POINTER(KvCache), C.POINTER(KvPool), C.c_void_p, C.c_void_p, C.c_void_p]),
+    "b200q_kv_compact_dev": (C.c_int, [C.POINTER(KvCache), C.POINTER(KvPool), C.c_void_p, C.c_int64, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p]),
+    "b200q_rope_plan_init": (C.c_int, [C.POINTER(RopePlan), C.c_int32, C.c_int32, C.c_int32, C.c_double, C.POINTER(RopeScaling)]),
+    "b200q_rope_dev": (C.c_int, [C.POINTER(RopePlan), C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_int32] + [C.c_int64] * 4 +
+                       [C.c_int32, C.c_void_p]),
+    "b200q_rope_append_dev": (C.c_int, [C.POINTER(RopePlan), C.POINTER(KvCache), C.POINTER(KvPool), C.POINTER(RopeAppend), C.c_void_p]),
+    "b200q_tree_attention_workspace": (C.c_int, [C.POINTER(KvCache), C.c_int32, C.POINTER(C.c_int64)]),
+    "b200q_tree_attention_dev": (C.c_int, [C.POINTER(KvCache), C.POINTER(KvPool), C.POINTER(TreeAttention), C.c_void_p]),
     "kl_diversity_hist": (C.c_float, [C.POINTER(C.c_int), C.c_float, C.c_longlong, C.c_longlong]),
     "kl_diversity": (C.c_float, [C.POINTER(C.c_float), C.c_longlong, C.c_longlong]),
     "b200q_conv2d_dev_set_profiling": (C.c_int, [C.c_void_p, C.c_int]),
