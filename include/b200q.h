@@ -610,7 +610,7 @@ int b200q_top_distance_f32_dev(const float *x, const float *ref, int64_t count, 
 
 /* Keys and values: element (layer, page, slot, head, d) of either lies at layer * layer_stride + page * page_stride +
  * slot * slot_stride + head * head_stride + d, in elements; any order of the dimensions.  k, v 16-byte aligned, strides
- * multiples of 8 elements, head_dim a multiple of 8 up to 256, dtype B200Q_DT_BF16 or B200Q_DT_F16.  The number of pages and
+ * positive multiples of 8 elements, head_dim a multiple of 8 up to 256, dtype B200Q_DT_BF16 or B200Q_DT_F16.  The number of pages and
  * of slots in a page stand in the pool. */
 typedef struct {
   void *k, *v;
@@ -723,6 +723,7 @@ typedef struct {
   int64_t rows;
   int32_t q_heads, layer;
   float scale;
+  int32_t *status;           /* optional: receives a non-zero code if a bounded wait in the kernel ran out */
 } b200q_tree_attention;
 /* The workspace's size for this cache's head size on the device that holds the cache. */
 int b200q_tree_attention_workspace(const b200q_kv_cache *cache, int32_t q_heads, int64_t *bytes);

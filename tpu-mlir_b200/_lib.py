@@ -123,7 +123,7 @@ class TreeAttention(C.Structure):
     """b200q_tree_attention: the rows that attend and their masks."""
     _fields_ = [(n, C.c_void_p) for n in ("q", "out", "row_start", "mask", "workspace")] + [("workspace_bytes", C.c_int64)] + \
                [(n, C.c_int64) for n in ("q_row_stride", "q_head_stride", "out_row_stride", "out_head_stride", "mask_stride", "rows")] + \
-               [("q_heads", C.c_int32), ("layer", C.c_int32), ("scale", C.c_float)]
+               [("q_heads", C.c_int32), ("layer", C.c_int32), ("scale", C.c_float), ("status", C.c_void_p)]
 
 
 _FLOATPP = C.POINTER(C.POINTER(C.c_float))

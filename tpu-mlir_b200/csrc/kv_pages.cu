@@ -37,6 +37,9 @@ int kv_check_cache(const char* who, const b200q_kv_cache* cache) {
   if (c.heads > 65535 || c.layers > 65535) return set_error(B200Q_ERR_UNSUPPORTED, "%s: at most 65535 heads and layers", who);
   if ((c.layer_stride | c.page_stride | c.slot_stride | c.head_stride) & 7)
     return set_error(B200Q_ERR_INVALID, "%s: the cache's strides must be multiples of 8 elements", who);
+  if (c.layer_stride < 0 || c.page_stride < 1 || c.slot_stride < 1 || c.head_stride < 1 || c.page_stride >= 1LL << 38 ||
+      c.slot_stride >= 1LL << 38 || c.head_stride >= 1LL << 38)
+    return set_error(B200Q_ERR_INVALID, "%s: the cache's strides must be positive (and below 2^38 elements)", who);
   return B200Q_OK;
 }
 

@@ -4,19 +4,22 @@
 //   the drafted nodes that its mask names.
 //
 // One pass over keys and values with a running maximum and sum.  The heads that share a cache head are stacked: its rows are
-// (node, head of the group), 16, 32 or 64 of them in a tile, so that a key is read once for all of them.  Work is counted in units of
+// (node, head of the group), 16 or 32 of them in a tile, so that a key is read once for all of them.  Work is counted in units of
 // 64 positions of one (sequence, cache head, row tile); the units of the whole batch stand in one line and every block takes an
 // equal run of them, so uneven contexts do not wait for each other and one long context fills the GPU.  Lengths stay on the
 // device: each block adds up the batch's units for itself.  An item that a run's end cuts leaves fp32 partial sums in the workspace
 // (at most two a block), which a second kernel joins, in the order of the positions.
 //
-// Loads run ahead of the products across items: a ring of stages of 64 keys and values, filled with 16-byte cp.async through
-// the page table, whose entries are looked up one unit earlier.  Shared memory is swizzled by 16-byte pieces (piece ^ row % 8),
-// so that ldmatrix meets no bank twice.
+// One warp of a block only loads, with TMA boxes of as many rows as both a page and a unit are made of: a lane looks a box's page
+// up and issues its copy, ahead of the products and across items, into a ring of stages of 64 keys and values; four warps
+// compute.  Shared memory holds 64 elements a row, swizzled by 16-byte pieces (piece ^ row % 8), so that ldmatrix meets no bank
+// twice.  (Loading with 16-byte cp.async instead, one or two warps a block, took 640 instructions a warp and unit and held the
+// computing warps up: 108 us where this takes %%%.)
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <math.h>
 
+#include "igemm.h"
 #include "kv_cache.h"
 #include "ptx_sm100.cuh"
 
@@ -31,7 +34,10 @@ struct AttnArgs {
   b200q_tree_attention io;
   int group;          // query heads of a cache head
   float scale_log2;   // scale * log2(e)
-  int min_units;      // units that a block takes at least, if there are any
+  int box;            // rows of a TMA box
+  int min_run;        // the shortest run of the line that a block takes, if there is so much
+  unsigned long long wait_ns;   // no wait inside the kernel lasts longer
+  int expect_extra;             // test aid: bytes that a stage waits for and that never come (0 in normal use)
   float* partial;     // [blocks][2][rows of a tile][dim + 2]: sums, maximum (log2 domain), total
   struct SplitItem* items;   // [blocks]
 };
@@ -59,14 +65,11 @@ __device__ __forceinline__ Sequence load_sequence(const AttnArgs& a, int s) {
   return q;
 }
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool there) {
-  const int n = there ? 16 : 0;   // 0: the 16 bytes become zeros, nothing is read
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+// a box of a page's rows: x byte of the head, y slot, z head, w page; what lies outside becomes zeros
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z, int w) {
+  asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
+               "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z), "r"(w)
+               : "memory");
 }
 __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
@@ -118,11 +121,12 @@ __device__ __forceinline__ float from_bits(uint32_t bits) {
 __device__ __forceinline__ uint64_t low_bits(int n) { return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1; }
 
 // Which of the 64 positions from `p0` on node `node` sees: all committed ones, and the nodes that its mask names (a chain: up to
-// itself).  mask: the row's words.
-__device__ __forceinline__ uint64_t sees(const AttnArgs& a, const uint32_t* mask, int node, int length, int p0) {
+// itself).
+__device__ __forceinline__ uint64_t sees(const AttnArgs& a, int row, int node, int length, int p0) {
   const int base = p0 - length;   // node at the first position, negative: committed
   if (base <= -64) return ~0ull;
   if (!a.io.mask) return low_bits(node - base + 1);
+  const uint32_t* mask = a.io.mask + (int64_t)row * a.io.mask_stride;
   const int from = base > 0 ? base : 0;
   const int64_t w = from >> 5;
   const int sh = from & 31;
@@ -133,43 +137,72 @@ __device__ __forceinline__ uint64_t sees(const AttnArgs& a, const uint32_t* mask
   return base >= 0 ? bits : low_bits(-base) | bits << -base;
 }
 
-template <int DIM, int WR, int WC>
-struct Shape {
-  static constexpr int ROWS = 16 * WR, THREADS = 32 * WR * WC, STAGES = DIM > 128 ? 2 : 3, COLS = UNIT / WC;
-  static constexpr int TILE = UNIT * DIM * 2;                         // bytes of a stage's keys, and of its values
-  static constexpr int MERGE = WC > 1 ? ROWS * 64 * 4 + 2 * WC * ROWS * 4 : 0;
-  static constexpr int FIXED = STAGES * 2 * TILE + MERGE;
-  static size_t bytes(int sequences) { return FIXED + (size_t)sequences * (sizeof(long long) + sizeof(Sequence)); }
+// ---- the line of units: which unit stands at a position of it
+struct Line {
+  const Sequence* seqs;
+  int sequences, heads, group, tile_rows;
+};
+// An item (sequence, cache head, row tile) takes ITEM_COST positions of the line and one for each unit: what a block spends on an
+// item besides its units (queries, the sums' way out) counts when runs are made equal.
+constexpr int ITEM_COST = 1;
+struct Place {
+  long long pos;                     // in the line
+  int s, head, tile, unit;           // row tile of the sequence, unit of the item
+  int tiles, units, total, length, nodes, first_row;
+  __device__ __forceinline__ void enter(const Line& line, int seq) {
+    const Sequence q = line.seqs[seq];
+    s = seq;
+    tiles = (int)(((long long)q.nodes * line.group + line.tile_rows - 1) / line.tile_rows);
+    units = (q.total + UNIT - 1) / UNIT;
+    total = q.total;
+    length = q.length;
+    nodes = q.nodes;
+    first_row = q.first_row;
+  }
+  // the unit at `pos` or the first one after it; sums: the line's length up to and with each sequence
+  __device__ __forceinline__ void find(const Line& line, const long long* sums, long long at) {
+    int lo = 0, hi = line.sequences - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (sums[mid] > at) hi = mid;
+      else lo = mid + 1;
+    }
+    enter(line, lo);
+    const long long local = at - (lo ? sums[lo - 1] : 0), item = local / (units + ITEM_COST);
+    const int in = (int)(local - item * (units + ITEM_COST)) - ITEM_COST;
+    head = (int)(item / tiles);
+    tile = (int)(item - (long long)head * tiles);
+    unit = in > 0 ? in : 0;
+    pos = at + (in < 0 ? -in : 0);
+  }
+  // row tiles of a head stand next to each other: they read the same keys
+  __device__ __forceinline__ void next(const Line& line) {
+    ++pos;
+    if (++unit < units) return;
+    unit = 0;
+    pos += ITEM_COST;
+    if (++tile < tiles) return;
+    tile = 0;
+    if (++head < line.heads) return;
+    head = 0;
+    int q = s + 1;
+    while (q < line.sequences && line.seqs[q].nodes == 0) ++q;
+    if (q < line.sequences) enter(line, q);
+  }
 };
 
-// DIM: head size that the registers and the tiles are laid out for (head_dim <= DIM; pieces past it stay zero).
-// WR x WC warps: WR take 16 rows each, WC share a unit's positions.
-template <bool F16, int DIM, int WR, int WC>
-__global__ void __launch_bounds__(32 * WR * WC) tree_attention_kernel(const __grid_constant__ AttnArgs a) {
-  using S = Shape<DIM, WR, WC>;
-  constexpr int STAGES = S::STAGES, THREADS = S::THREADS, NT = S::COLS / 8, PIECES = DIM / 8, SLOTS = STAGES + 1;
-  extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ int64_t offset[SLOTS][UNIT];        // element offset of a unit's rows in keys and values, -1: none
-  __shared__ uint32_t there[SLOTS][2];           // which rows have one
-  __shared__ long long scan_buf[33];
-  __shared__ uint32_t bad[2];                    // rows of the unit whose values hold infinities or NaN
-  float* merge = reinterpret_cast<float*>(smem + STAGES * 2 * S::TILE);
-  float* merge_ml = merge + S::ROWS * 64;
-  long long* sums = reinterpret_cast<long long*>(smem + S::FIXED);
-  Sequence* seqs = reinterpret_cast<Sequence*>(sums + a.pool.sequences);
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, wr = warp / WC, wc = warp % WC;
-  const int n = a.pool.sequences, dim = a.cache.head_dim, heads = a.cache.heads, group = a.group;
-  ptx::griddep_launch_dependents();
-
-  // ---- the batch's units, sequence by sequence
+// Fills seqs and sums (the line's length up to and with each sequence) for all threads of the block; returns the line's length.
+template <int THREADS>
+__device__ __forceinline__ long long lay_out(const AttnArgs& a, int tile_rows, Sequence* seqs, long long* sums, long long* buf) {
+  const int n = a.pool.sequences, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int each = (n + THREADS - 1) / THREADS;
   long long mine = 0;
   for (int i = 0; i < each; ++i) {
     const int s = tid * each + i;
     if (s >= n) break;
     const Sequence q = load_sequence(a, s);
-    const long long tiles = ((long long)q.nodes * group + S::ROWS - 1) / S::ROWS;
-    mine += heads * tiles * ((q.total + UNIT - 1) / UNIT);
+    const long long tiles = ((long long)q.nodes * a.group + tile_rows - 1) / tile_rows;
+    mine += a.cache.heads * tiles * ((q.total + UNIT - 1) / UNIT + ITEM_COST);
     seqs[s] = q;
     sums[s] = mine;
   }
@@ -179,132 +212,190 @@ __global__ void __launch_bounds__(32 * WR * WC) tree_attention_kernel(const __gr
     const long long o = __shfl_up_sync(0xffffffffu, upto, d);
     if (lane >= d) upto += o;
   }
-  if (lane == 31) scan_buf[warp] = upto;
-  if (tid < 2) bad[tid] = 0;
-  // pieces past head_dim are never loaded: zero once
-  for (int i = tid; i < STAGES * 2 * UNIT * PIECES; i += THREADS)
-    if (i % PIECES >= dim / 8) {
-      const int row = i / PIECES % UNIT, piece = i % PIECES;
-      *reinterpret_cast<uint4*>(smem + (i / (PIECES * UNIT)) * S::TILE + row * DIM * 2 + ((piece ^ (row & 7)) * 16)) = make_uint4(0, 0, 0, 0);
-    }
+  if (lane == 31) buf[warp] = upto;
   __syncthreads();
   long long before = upto - mine, total = 0;
 #pragma unroll
-  for (int w = 0; w < WR * WC; ++w) {
-    if (w < warp) before += scan_buf[w];
-    total += scan_buf[w];
+  for (int w = 0; w < THREADS / 32; ++w) {
+    if (w < warp) before += buf[w];
+    total += buf[w];
   }
   for (int i = 0; i < each; ++i)
     if (tid * each + i < n) sums[tid * each + i] += before;
   __syncthreads();
+  return total;
+}
+
+// ---- loading.  Layout of a tile: [64 elements of the head][row][128 bytes], 16-byte pieces swizzled by the row.
+__device__ __forceinline__ uint32_t tile_at(int row, int piece) {
+  return (piece >> 3) * (UNIT * 128) + row * 128 + (((piece & 7) ^ (row & 7)) * 16);
+}
+// The loading warp's life: every unit of the block's run into the ring.  A box is `box` rows (the greatest common divisor of a page's
+// and a unit's, so no box is cut by either) of 64 elements.  there[stage]: rows that are positions of the sequence in a page of the pool
+// (the others are zeros, or whatever a page holds past the sequence's end).
+template <int DIM, int STAGES, typename Wait>
+__device__ __forceinline__ void load_units(const AttnArgs& a, const CUtensorMap* km, const CUtensorMap* vm, const Line& line, Place at, long long end,
+                                           uint8_t* ring, uint64_t* full_bar, uint64_t* empty_bar, uint64_t* there, Wait wait) {
+  constexpr int TILE = UNIT * DIM * 2, PARTS = 2 * (DIM / 64);
+  const int lane = threadIdx.x & 31, box = a.box, boxes = UNIT / box, page_size = a.pool.page_size;
+  int stage = 0;
+  uint32_t phase = 1, sent = 0;   // the first pass over the ring finds it empty
+  // the place of box `lane` (and lane + 32) of the unit that `at` stands at: page (-1: none) and slot of its first row
+  int page[2], slot[2], rows;
+  auto look_up = [&]() {
+    rows = at.total - at.unit * UNIT;   // may be more than a unit's
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int b = lane + 32 * j, pos = at.unit * UNIT + b * box;
+      page[j] = -1;
+      slot[j] = 0;
+      if (b < boxes && pos < at.total) {
+        page[j] = kv_page(a.pool, at.s, pos);
+        slot[j] = (int)((unsigned)pos % (unsigned)page_size);
+      }
+    }
+  };
+  look_up();
+  while (at.pos < end) {
+    const int head = at.head, pg0 = page[0], pg1 = page[1], sl0 = slot[0], sl1 = slot[1], here = rows;
+    at.next(line);
+    if (at.pos < end) look_up();   // the next unit's entries are on their way while this one's boxes go out
+    if (!wait(&empty_bar[stage], phase, 1)) break;
+    ++sent;
+    uint64_t in = 0;
+    if (pg0 >= 0) in |= low_bits(box) << (lane * box);
+    if (pg1 >= 0) in |= low_bits(box) << ((lane + 32) * box);
+    in = (uint64_t)__reduce_or_sync(0xffffffffu, (uint32_t)(in >> 32)) << 32 | __reduce_or_sync(0xffffffffu, (uint32_t)in);
+    const uint32_t bar = ptx::smem_u32(&full_bar[stage]), dst = ptx::smem_u32(ring) + stage * 2 * TILE;
+    if (lane == 0) {
+      there[stage] = in & low_bits(here);
+      ptx::mbar_arrive_expect_tx(bar, 2 * TILE + a.expect_extra);
+    }
+    __syncwarp();
+    // a copy a lane: box, then keys or values and which 64 elements
+    for (int i = lane; i - lane < boxes * PARTS; i += 32) {
+      const int b = i / PARTS, part = i % PARTS;
+      const int p0 = __shfl_sync(0xffffffffu, pg0, b & 31), p1 = __shfl_sync(0xffffffffu, pg1, b & 31);
+      const int s0 = __shfl_sync(0xffffffffu, sl0, b & 31), s1 = __shfl_sync(0xffffffffu, sl1, b & 31);
+      if (b < boxes) {
+        const int pg = b < 32 ? p0 : p1, sl = b < 32 ? s0 : s1, x = part >> 1;
+        tma_load_4d(dst + (part & 1) * TILE + x * (UNIT * 128) + b * box * 128, part & 1 ? vm : km, bar, x * 128, sl, head, pg < 0 ? a.pool.pages : pg);
+      }
+    }
+    if (++stage == STAGES) {
+      stage = 0;
+      phase ^= 1;
+    }
+  }
+  if (at.pos < end) {
+    // given up: what is still on its way lands before the block is gone
+    int flag = 0;
+    for (uint32_t i = 0; i < STAGES; ++i)
+      if (i < sent) ptx::mbar_wait_bounded(ptx::smem_u32(&full_bar[i]), ((sent - i - 1) / STAGES) & 1, &flag, 1, a.wait_ns);
+  }
+}
+
+constexpr int COMPUTERS = 128, BLOCK = COMPUTERS + 32;
+
+__device__ __forceinline__ void computers_sync() { asm volatile("barrier.cta.sync 1, 128;" ::: "memory"); }
+__device__ __forceinline__ bool computers_or(bool x) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p, q;\n\t"
+      "setp.ne.b32 q, %1, 0;\n\t"
+      "barrier.cta.red.or.pred p, 1, 128, q;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t"
+      "}\n"
+      : "=r"(r)
+      : "r"((uint32_t)x)
+      : "memory");
+  return r != 0;
+}
+
+template <int DIM, int WR, int WC>
+struct Shape {
+  static constexpr int ROWS = 16 * WR, STAGES = DIM > 128 ? 2 : 3, COLS = UNIT / WC;
+  static constexpr int TILE = UNIT * DIM * 2;                         // bytes of a stage's keys, and of its values
+  static constexpr int MERGE = WC > 1 ? ROWS * 64 * 4 + 2 * WC * ROWS * 4 : 0;
+  static constexpr int FIXED = STAGES * 2 * TILE + MERGE;
+  static size_t bytes(int sequences) { return 1024 + FIXED + (size_t)sequences * (sizeof(long long) + sizeof(Sequence)); }
+};
+
+// DIM: head size that the registers and the tiles are laid out for (head_dim <= DIM; pieces past it stay zero).
+// WR x WC computing warps: WR take 16 rows each, WC share a unit's positions.
+template <bool F16, int DIM, int WR, int WC>
+__global__ void __launch_bounds__(BLOCK, DIM > 128 ? 1 : 2)
+tree_attention_kernel(const __grid_constant__ CUtensorMap km, const __grid_constant__ CUtensorMap vm, const __grid_constant__ AttnArgs a) {
+  using S = Shape<DIM, WR, WC>;
+  static_assert(WR * WC * 32 == COMPUTERS, "");
+  constexpr int STAGES = S::STAGES, NT = S::COLS / 8, PIECES = DIM / 8;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + (-ptx::smem_u32(smem_raw) & 1023);   // the swizzle goes by the address
+  __shared__ uint64_t there[STAGES];             // which rows of a unit are positions with a page
+  __shared__ long long scan_buf[BLOCK / 32];
+  __shared__ uint32_t bad[2];                    // rows of the unit whose values hold infinities or NaN
+  __shared__ alignas(8) uint64_t full_bar[STAGES], empty_bar[STAGES];
+  __shared__ int abort_flag;
+  float* merge = reinterpret_cast<float*>(smem + STAGES * 2 * S::TILE);
+  float* merge_ml = merge + S::ROWS * 64;
+  long long* sums = reinterpret_cast<long long*>(smem + S::FIXED);
+  Sequence* seqs = reinterpret_cast<Sequence*>(sums + a.pool.sequences);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int dim = a.cache.head_dim, group = a.group;
+  ptx::griddep_launch_dependents();
+
+  if (tid == 0) {
+    for (int i = 0; i < STAGES; ++i) {
+      ptx::mbar_init(ptx::smem_u32(&full_bar[i]), 1);
+      ptx::mbar_init(ptx::smem_u32(&empty_bar[i]), COMPUTERS / 32);
+    }
+    ptx::fence_barrier_init();
+    abort_flag = 0;
+    bad[0] = bad[1] = 0;
+  }
+  const long long total = lay_out<BLOCK>(a, S::ROWS, seqs, sums, scan_buf);
+  const Line line{seqs, a.pool.sequences, a.cache.heads, group, S::ROWS};
 
   long long run = (total + gridDim.x - 1) / gridDim.x;
-  if (run < a.min_units) run = a.min_units;
+  if (run < a.min_run) run = a.min_run;
   const long long u0 = (long long)blockIdx.x * run, u1 = u0 + run < total ? u0 + run : total;
   if (tid == 0) a.items[blockIdx.x].parts = 0;
   if (u0 >= u1) return;
-
-  // ---- where the loads are: unit `u` of the line
-  struct Place {
-    int s, head, tile, unit, tiles, units;   // row tile, unit of the item; how many there are
-    int total, length, nodes, first_row;
-  };
-  auto enter = [&](Place& p, int s) {
-    const Sequence q = seqs[s];
-    p.s = s;
-    p.tiles = (q.nodes * group + S::ROWS - 1) / S::ROWS;
-    p.units = (q.total + UNIT - 1) / UNIT;
-    p.total = q.total;
-    p.length = q.length;
-    p.nodes = q.nodes;
-    p.first_row = q.first_row;
-  };
-  auto next_item = [&](Place& p) {   // row tiles of a head next to each other: they read the same keys
-    p.unit = 0;
-    if (++p.tile < p.tiles) return;
-    p.tile = 0;
-    if (++p.head < heads) return;
-    p.head = 0;
-    int s = p.s + 1;
-    while (s < n && seqs[s].nodes == 0) ++s;
-    if (s < n) enter(p, s);
-  };
-  Place load;
-  {
-    int lo = 0, hi = n - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi) >> 1;
-      if (sums[mid] > u0) hi = mid;
-      else lo = mid + 1;
-    }
-    enter(load, lo);
-    const long long local = u0 - (lo ? sums[lo - 1] : 0), item = local / load.units;
-    load.unit = (int)(local - item * load.units);
-    load.head = (int)(item / load.tiles);
-    load.tile = (int)(item - (long long)load.head * load.tiles);
-  }
-  Place at = load;
-  const int count = (int)(u1 - u0);
-
-  // the offset of row `tid` of the unit that `load` stands at, which then goes one further
-  auto look_up = [&]() -> int64_t {
-    int64_t off = -1;
-    if (tid < UNIT) {
-      const int pos = load.unit * UNIT + tid;
-      if (pos < load.total) {
-        off = kv_entry(a.cache, a.pool, load.s, pos);
-        if (off >= 0) off += load.head * a.cache.head_stride;
-      }
-    }
-    if (++load.unit == load.units) next_item(load);
-    return off;
-  };
-  auto note = [&](int slot, int64_t off) {
-    if (tid < UNIT) {
-      offset[slot][tid] = off;
-      const uint32_t m = __ballot_sync(0xffffffffu, off >= 0);
-      if (lane == 0) there[slot][warp] = m;
-    }
-  };
-  const uint16_t* kp = static_cast<const uint16_t*>(a.cache.k) + a.io.layer * a.cache.layer_stride;
+  Place at;
+  at.find(line, sums, u0);
   const uint16_t* vp = static_cast<const uint16_t*>(a.cache.v) + a.io.layer * a.cache.layer_stride;
   const uint32_t smem_base = ptx::smem_u32(smem);
-  auto fetch = [&](int stage, int slot) {
-    const int piece = tid % PIECES;
-    if (piece < dim / 8) {
-#pragma unroll
-      for (int i = 0; i < UNIT * PIECES / THREADS; ++i) {
-        const int row = tid / PIECES + i * (THREADS / PIECES);
-        const int64_t off = offset[slot][row];
-        const int64_t at16 = (off >= 0 ? off : 0) + piece * 8;
-        const uint32_t dst = smem_base + stage * 2 * S::TILE + row * DIM * 2 + ((piece ^ (row & 7)) * 16);
-        cp_async16(dst, kp + at16, off >= 0);
-        cp_async16(dst + S::TILE, vp + at16, off >= 0);
-      }
-    }
+  // A wait that runs out (it cannot, short of a fault) ends all waiting: the roles go on without, so that no barrier is left short,
+  // and the status says so.
+  bool dead = false;
+  auto wait = [&](uint64_t* bar, uint32_t parity, int where) {
+    if (!dead) dead = !ptx::mbar_wait_bounded(ptx::smem_u32(bar), parity, &abort_flag, where, a.wait_ns);
+    return !dead;
   };
 
-#pragma unroll
-  for (int i = 0; i < STAGES; ++i)
-    if (i < count) note(i, look_up());
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < STAGES - 1; ++i) {
-    if (i < count) fetch(i, i);
-    cp_async_commit();
+  if (warp >= COMPUTERS / 32) {
+    // ---------------------------------------------------------------- loading
+    load_units<DIM, STAGES>(a, &km, &vm, line, at, u1, smem, full_bar, empty_bar, there, wait);
+    if (dead && lane == 0 && a.io.status) atomicMax(a.io.status, abort_flag);
+    return;
   }
 
-  // ---- registers: queries (A fragments), sums, running maximum (log2 domain) and total of rows lane / 4 and lane / 4 + 8
+  // ------------------------------------------------------------------ computing
+  const int wr = warp / WC, wc = warp % WC;
+  // queries (A fragments), sums, running maximum (log2 domain) and total of rows lane / 4 and lane / 4 + 8
   uint32_t q[DIM / 16][4];
   float o[DIM / 8][4], m[2], l[2];
-  const uint32_t* mask[2];
   int node[2];
-  int started = at.unit;   // unit of the item that this block's part starts with
-  int stage = 0, slot = 0;
+  int started = 0;   // unit of the item that this block's part starts with
+  bool fresh = true;
+  int stage = 0;
+  uint32_t phase = 0;
 
-  for (int i = 0; i < count; ++i) {
-    if (i == 0 || at.unit == 0) {
+  while (at.pos < u1) {
+    if (fresh) {
       // a new item (or this block's part of one)
+      fresh = false;
       started = at.unit;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -312,7 +403,6 @@ __global__ void __launch_bounds__(32 * WR * WC) tree_attention_kernel(const __gr
         const bool real = r < at.nodes * group;
         const int t = r / group, row = at.first_row + (real ? t : 0);
         node[h] = t;
-        mask[h] = a.io.mask ? a.io.mask + (int64_t)row * a.io.mask_stride : nullptr;
         m[h] = -INFINITY;
         l[h] = 0.f;
         const uint16_t* src = static_cast<const uint16_t*>(a.io.q) + (int64_t)row * a.io.q_row_stride + (at.head * group + r % group) * a.io.q_head_stride;
@@ -328,16 +418,13 @@ __global__ void __launch_bounds__(32 * WR * WC) tree_attention_kernel(const __gr
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[k][e] = 0.f;
     }
-
-    cp_async_wait<STAGES - 2>();
-    __syncthreads();   // unit i is here, and every warp is done with unit i - 1
-    if (i + STAGES - 1 < count) fetch((stage + STAGES - 1) % STAGES, (slot + STAGES - 1) % SLOTS);
-    cp_async_commit();
-    int64_t ahead = -1;
-    if (i + STAGES < count) ahead = look_up();
+    wait(&full_bar[stage], phase, 2);
 
     // ---- scores of 16 rows x COLS positions
+    // (pieces 2k and 2k + 1 of a row: the swizzle makes the step from k to k + 1 an exclusive or of 32 bytes)
     const uint32_t ks = smem_base + stage * 2 * S::TILE, vs = ks + S::TILE;
+    const uint32_t k_lane = ks + tile_at(wc * S::COLS + (lane >> 4) * 8 + (lane & 7), (lane >> 3) & 1);
+    const uint32_t v_lane = vs + tile_at(wc * S::COLS + ((lane >> 3) & 1) * 8 + (lane & 7), lane >> 4);
     float sc[NT][4];
 #pragma unroll
     for (int t = 0; t < NT; ++t)
@@ -349,8 +436,7 @@ __global__ void __launch_bounds__(32 * WR * WC) tree_attention_kernel(const __gr
 #pragma unroll
         for (int t = 0; t < NT; t += 2) {
           uint32_t b[4];
-          const int row = wc * S::COLS + t * 8 + (lane >> 4) * 8 + (lane & 7), piece = k * 2 + ((lane >> 3) & 1);
-          ldmatrix4(b, ks + row * DIM * 2 + ((piece ^ (row & 7)) * 16));
+          ldmatrix4(b, ((k_lane + t * 8 * 128) ^ ((k & 3) * 32)) + (k >> 2) * (UNIT * 128));
           mma16816<F16>(sc[t], q[k], b[0], b[1]);
           mma16816<F16>(sc[t + 1], q[k], b[2], b[3]);
         }
@@ -359,14 +445,14 @@ __global__ void __launch_bounds__(32 * WR * WC) tree_attention_kernel(const __gr
 
     // ---- what is not seen
     const int p0 = at.unit * UNIT;
-    const uint64_t in_pool = (uint64_t)there[slot][1] << 32 | there[slot][0];
+    const uint64_t in_pool = there[stage];
     const bool drafted = p0 + UNIT > at.length;
     uint64_t see[2] = {~0ull, ~0ull};
     bool fix = false;
     if (drafted || in_pool != ~0ull) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        see[h] = in_pool & sees(a, mask[h], node[h], at.length, p0);
+        see[h] = in_pool & sees(a, at.first_row + (node[h] < at.nodes ? node[h] : 0), node[h], at.length, p0);
         const uint64_t mine64 = see[h] >> (wc * S::COLS + (lane & 3) * 2);
 #pragma unroll
         for (int t = 0; t < NT; ++t)
@@ -377,22 +463,22 @@ __global__ void __launch_bounds__(32 * WR * WC) tree_attention_kernel(const __gr
       if (drafted) {
         // Values of drafted nodes meet weights of zero in rows that do not see them: infinite or NaN ones are taken out of the
         // tile (and added below where they are seen), or they would make those rows NaN.
-        int found = 0;
-        for (int c = tid; c < UNIT * PIECES; c += THREADS) {
-          const int row = c / PIECES, piece = c % PIECES;
-          uint32_t* w = reinterpret_cast<uint32_t*>(smem + (vs - smem_base) + row * DIM * 2 + ((piece ^ (row & 7)) * 16));
+        bool found = false;
+        for (int c = tid; c < UNIT * PIECES; c += COMPUTERS) {
+          const int row = c / PIECES;
+          uint32_t* w = reinterpret_cast<uint32_t*>(smem + (vs - smem_base) + tile_at(row, c % PIECES));
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const uint32_t x = w[j];
             const bool lo = not_finite<F16>(x & 0xffffu), hi = not_finite<F16>(x >> 16);
             if (lo || hi) {
-              found = 1;
+              found = true;
               w[j] = (lo ? 0u : x & 0xffffu) | (hi ? 0u : x & 0xffff0000u);
               atomicOr(&bad[row >> 5], 1u << (row & 31));
             }
           }
         }
-        fix = __syncthreads_or(found);
+        fix = computers_or(found);
       }
     }
 
@@ -439,8 +525,7 @@ __global__ void __launch_bounds__(32 * WR * WC) tree_attention_kernel(const __gr
       for (int k = 0; k < DIM / 16; ++k) {
         if (k * 16 < dim) {
           uint32_t b[4];
-          const int row = wc * S::COLS + j * 16 + ((lane >> 3) & 1) * 8 + (lane & 7), piece = k * 2 + (lane >> 4);
-          ldmatrix4_t(b, vs + row * DIM * 2 + ((piece ^ (row & 7)) * 16));
+          ldmatrix4_t(b, ((v_lane + j * 16 * 128) ^ ((k & 3) * 32)) + (k >> 2) * (UNIT * 128));
           mma16816<F16>(o[2 * k], p, b[0], b[1]);
           mma16816<F16>(o[2 * k + 1], p, b[2], b[3]);
         }
@@ -462,12 +547,13 @@ __global__ void __launch_bounds__(32 * WR * WC) tree_attention_kernel(const __gr
         const int from = (lane & ~3) | ((c & 7) >> 1);
         w[0] = __shfl_sync(0xffffffffu, w[0], from);
         w[1] = __shfl_sync(0xffffffffu, w[1], from);
-        const int64_t off = offset[slot][row];
-        if (off < 0) continue;
+        const int64_t entry = kv_entry(a.cache, a.pool, at.s, p0 + row);
+        if (entry < 0) continue;
+        const uint16_t* value = vp + entry + at.head * a.cache.head_stride;
 #pragma unroll
         for (int k = 0; k < DIM / 8; ++k) {
           const int d = k * 8 + (lane & 3) * 2;
-          const uint32_t x = d < dim ? *reinterpret_cast<const uint32_t*>(vp + off + d) : 0u;
+          const uint32_t x = d < dim ? *reinterpret_cast<const uint32_t*>(value + d) : 0u;
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             const uint32_t v = e ? x >> 16 : x & 0xffffu;
@@ -478,15 +564,22 @@ __global__ void __launch_bounds__(32 * WR * WC) tree_attention_kernel(const __gr
           }
         }
       }
-      __syncthreads();
-      if (tid < 2) bad[tid] = 0;
+      computers_sync();
+      if (tid < 2) bad[tid] = 0;   // (before anyone looks for the next unit's: that ends in a barrier, and starts with one wait more)
+      computers_sync();
     }
-    if (i + STAGES < count) note((slot + STAGES) % SLOTS, ahead);
-    stage = (stage + 1) % STAGES;
-    slot = (slot + 1) % SLOTS;
+    __syncwarp();
+    if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&empty_bar[stage]));
+    if (++stage == STAGES) {
+      stage = 0;
+      phase ^= 1;
+    }
 
     // ---- the end of the item, or of this block's part
-    if (++at.unit == at.units || i + 1 == count) {
+    const bool done = at.unit + 1 == at.units;
+    const long long first = at.pos - at.unit;   // where the item's units start in the line
+    if (done || at.pos + 1 == u1) {
+      fresh = true;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
@@ -494,7 +587,7 @@ __global__ void __launch_bounds__(32 * WR * WC) tree_attention_kernel(const __gr
       }
       if (WC > 1) {
         // the warps that shared the positions: a common maximum, then their sums one after the other, 64 columns at a time
-        __syncthreads();   // (the buffer may still be read for the item before)
+        computers_sync();   // (the buffer may still be read for the item before)
         if ((lane & 3) == 0)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
@@ -502,7 +595,7 @@ __global__ void __launch_bounds__(32 * WR * WC) tree_attention_kernel(const __gr
             merge_ml[wc * S::ROWS + r] = m[h];
             merge_ml[(WC + wc) * S::ROWS + r] = l[h];
           }
-        __syncthreads();
+        computers_sync();
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const int r = wr * 16 + lane / 4 + 8 * h;
@@ -540,11 +633,11 @@ __global__ void __launch_bounds__(32 * WR * WC) tree_attention_kernel(const __gr
                 if (w < WC - 1) buf[k * 32 + lane] = make_float4(x[0], x[1], x[2], x[3]);
               }
             }
-            __syncthreads();
+            computers_sync();
           }
         }
       }
-      const bool whole = started == 0 && at.unit == at.units;
+      const bool whole = started == 0 && done;
       if (wc == WC - 1) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -567,14 +660,12 @@ __global__ void __launch_bounds__(32 * WR * WC) tree_attention_kernel(const __gr
           }
         }
       }
-      if (tid == 0 && started == 0 && !whole) {
-        // the item's first unit is unit u1 - at.unit of the line
-        const long long last = u1 - at.unit + at.units - 1;
-        a.items[blockIdx.x] = SplitItem{(int)(last / run) - (int)blockIdx.x + 1, at.first_row, at.tile * S::ROWS, at.nodes * group, at.head};
-      }
-      if (at.unit == at.units) next_item(at);
+      if (tid == 0 && started == 0 && !whole)
+        a.items[blockIdx.x] = SplitItem{(int)((first + at.units - 1) / run) - (int)blockIdx.x + 1, at.first_row, at.tile * S::ROWS, at.nodes * group, at.head};
     }
+    at.next(line);
   }
+  if (dead && lane == 0 && a.io.status) atomicMax(a.io.status, abort_flag);
 }
 
 // Joins the parts of the items that were cut: block x looks after the item that starts in block x's run, a warp takes a row.
@@ -628,6 +719,14 @@ int64_t workspace_bytes(int blocks, int dim) {
 }
 int padded_dim(int head_dim) { return head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256; }
 
+// Keys or values of the layer as a TMA tensor [page][head][slot][bytes], boxes of `box` slots x 128 bytes.
+int make_map(CUtensorMap* map, const AttnArgs& a, const void* base) {
+  const uint64_t dims[4] = {(uint64_t)a.cache.head_dim * 2, (uint64_t)a.pool.page_size, (uint64_t)a.cache.heads, (uint64_t)a.pool.pages};
+  const uint64_t strides[3] = {(uint64_t)a.cache.slot_stride * 2, (uint64_t)a.cache.head_stride * 2, (uint64_t)a.cache.page_stride * 2};
+  const uint32_t box[4] = {128, (uint32_t)a.box, 1, 1};
+  return make_tmap_u8(map, static_cast<const uint16_t*>(base) + a.io.layer * a.cache.layer_stride, 4, dims, strides, box);
+}
+
 template <bool F16, int DIM, int WR, int WC>
 int launch(const AttnArgs& a, int sms, cudaStream_t s) {
   using S = Shape<DIM, WR, WC>;
@@ -635,7 +734,10 @@ int launch(const AttnArgs& a, int sms, cudaStream_t s) {
   const size_t smem = S::bytes(a.pool.sequences);
   CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::bytes(KV_MAX_SEQUENCES)));
   const int blocks = sms * (DIM > 128 ? 1 : BLOCKS_PER_SM);
-  kernel<<<blocks, S::THREADS, smem, s>>>(a);
+  CUtensorMap km, vm;
+  B200Q_TRY(make_map(&km, a, a.cache.k));
+  B200Q_TRY(make_map(&vm, a, a.cache.v));
+  kernel<<<blocks, BLOCK, smem, s>>>(km, vm, a);
   CUDA_TRY(cudaGetLastError());
   cudaLaunchAttribute attr;
   cudaLaunchConfig_t cfg = launch_config(dim3(blocks, S::ROWS / 4), dim3(128), 0, s, &attr, true);
@@ -648,8 +750,6 @@ template <bool F16, int DIM>
 int launch_rows(const AttnArgs& a, int sms, cudaStream_t s) {
   const int64_t rows = (a.io.rows + a.pool.sequences - 1) / a.pool.sequences * a.group;
   if (rows <= 16) return launch<F16, DIM, 1, 4>(a, sms, s);
-  if constexpr (DIM <= 128)
-    if (rows > 32) return launch<F16, DIM, 4, 1>(a, sms, s);
   return launch<F16, DIM, 2, 2>(a, sms, s);
 }
 
@@ -712,7 +812,10 @@ int b200q_tree_attention_dev(const b200q_kv_cache* cache, const b200q_kv_pool* p
   a.io = io;
   a.group = io.q_heads / cache->heads;
   a.scale_log2 = io.scale * 1.4426950408889634f;
-  a.min_units = 2;
+  a.box = UNIT;
+  while (pool->page_size % a.box) a.box /= 2;   // the greatest power of two that divides a page, up to a unit
+  igemm_wait_test(&a.expect_extra, &a.wait_ns);
+  a.min_run = 2 + ITEM_COST;
   a.items = static_cast<SplitItem*>(io.workspace);
   a.partial = reinterpret_cast<float*>(static_cast<uint8_t*>(io.workspace) + ((int64_t)blocks * sizeof(SplitItem) + 255) / 256 * 256);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
