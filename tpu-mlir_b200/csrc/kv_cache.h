@@ -32,22 +32,24 @@ class OnDeviceOf {
 // SMs of a device; negative when it cannot be asked.
 int sm_count(int device);
 
-// The launch that may start while its predecessor on the stream drains (every thread executes griddep_wait before it
-// touches what the predecessor wrote).
-inline cudaLaunchConfig_t launch_config(dim3 grid, dim3 block, size_t smem, cudaStream_t s, cudaLaunchAttribute* attr, bool dependent) {
+#ifdef __CUDACC__
+// Launches a kernel that may become resident while its predecessor on the stream drains: every thread of it executes griddep_wait
+// before it reads or writes anything outside the block, and it lets its own successor come early too.
+template <typename... Formal, typename... Actual>
+int launch_dependent(void (*kernel)(Formal...), dim3 grid, dim3 block, size_t smem, cudaStream_t s, Actual&&... args) {
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = grid;
   cfg.blockDim = block;
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
-  attr->id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr->val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = dependent ? 1 : 0;
-  return cfg;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, static_cast<Formal>(args)...));
+  return B200Q_OK;
 }
-
-#ifdef __CUDACC__
 // Page of position `pos` of sequence `s`, or -1 where the table has none in the pool.
 __device__ __forceinline__ int kv_page(const b200q_kv_pool& pool, int s, int pos) {
   const int j = (int)((unsigned)pos / (unsigned)pool.page_size);

@@ -196,6 +196,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) reserve_kernel(b200q_kv_pool poo
   __shared__ int base[KV_MAX_SEQUENCES];
   const int s = threadIdx.x;
   ptx::griddep_launch_dependents();
+  ptx::griddep_wait();
   long long need = 0;
   int held = 0, narrow = 0;
   if (s < pool.sequences && extra[s] >= 0) {
@@ -230,6 +231,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) reserve_kernel(b200q_kv_pool poo
 __global__ void __launch_bounds__(128) free_kernel(b200q_kv_pool pool, const int32_t* __restrict__ which) {
   const int s = blockIdx.x;
   ptx::griddep_launch_dependents();
+  ptx::griddep_wait();
   if (which[s] == 0) return;
   int n = pool.held[s];
   n = n < pool.table_width ? n : pool.table_width;
@@ -261,6 +263,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) fork_plan_kernel(b200q_kv_pool p
   const int s = threadIdx.x, n = pool.sequences;
   const ForkScratch f = fork_scratch(pool.scratch, n);
   ptx::griddep_launch_dependents();
+  ptx::griddep_wait();
   if (s < n) lengths[s] = kv_length(pool, s);
   __syncthreads();
   const int p = s < n ? parent[s] : -1;
@@ -305,8 +308,8 @@ fork_kernel(b200q_kv_cache cache, b200q_kv_pool pool, const int32_t* __restrict_
   __shared__ int32_t old[FORK_TILE];
   const int n = pool.sequences;
   const ForkScratch f = fork_scratch(pool.scratch, n);
-  ptx::griddep_wait();
   ptx::griddep_launch_dependents();
+  ptx::griddep_wait();
   if (*f.go == 0) return;
   if ((int)blockIdx.x < table_blocks) {
     for (int c0 = blockIdx.x * columns; c0 < pool.table_width; c0 += table_blocks * columns) {
@@ -363,6 +366,7 @@ compact_kernel(b200q_kv_cache cache, b200q_kv_pool pool, const int32_t* __restri
   __shared__ int good;
   const int parts = 2 * cache.layers, chunks = cache.head_dim / 8;
   ptx::griddep_launch_dependents();
+  ptx::griddep_wait();
   for (int item = blockIdx.x; item < pool.sequences * parts; item += gridDim.x) {
     const int s = item / parts, part = item % parts, length = kv_length(pool, s);
     int n = path_length[s];
@@ -399,8 +403,8 @@ compact_kernel(b200q_kv_cache cache, b200q_kv_pool pool, const int32_t* __restri
 
 // The new lengths take the place of the old ones once no block needs those.
 __global__ void __launch_bounds__(KV_MAX_SEQUENCES) lengths_kernel(const int32_t* __restrict__ from, int32_t* __restrict__ to, int n) {
-  ptx::griddep_wait();
   ptx::griddep_launch_dependents();
+  ptx::griddep_wait();
   if ((int)threadIdx.x < n) to[threadIdx.x] = from[threadIdx.x];
 }
 
@@ -434,9 +438,7 @@ int b200q_kv_reserve_dev(const b200q_kv_pool* pool, const int32_t* extra, int32_
   B200Q_TRY(dev.rc);
   size_t bytes;
   B200Q_TRY(bitmap_bytes((const void*)reserve_kernel, pool->pages, &bytes));
-  reserve_kernel<<<1, PLAN_THREADS, bytes, static_cast<cudaStream_t>(stream)>>>(*pool, extra, status);
-  CUDA_TRY(cudaGetLastError());
-  return B200Q_OK;
+  return launch_dependent(reserve_kernel, dim3(1), dim3(PLAN_THREADS), bytes, static_cast<cudaStream_t>(stream), *pool, extra, status);
 }
 
 int b200q_kv_free_dev(const b200q_kv_pool* pool, const int32_t* which, void* stream) {
@@ -445,9 +447,7 @@ int b200q_kv_free_dev(const b200q_kv_pool* pool, const int32_t* which, void* str
   if (pool->sequences == 0) return B200Q_OK;
   OnDeviceOf dev("kv_free", pool->table);
   B200Q_TRY(dev.rc);
-  free_kernel<<<pool->sequences, 128, 0, static_cast<cudaStream_t>(stream)>>>(*pool, which);
-  CUDA_TRY(cudaGetLastError());
-  return B200Q_OK;
+  return launch_dependent(free_kernel, dim3(pool->sequences), dim3(128), 0, static_cast<cudaStream_t>(stream), *pool, which);
 }
 
 int b200q_kv_fork_dev(const b200q_kv_cache* cache, const b200q_kv_pool* pool, const int32_t* parent, int32_t* status, void* stream) {
@@ -465,18 +465,14 @@ int b200q_kv_fork_dev(const b200q_kv_cache* cache, const b200q_kv_pool* pool, co
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   size_t bytes;
   B200Q_TRY(bitmap_bytes((const void*)fork_plan_kernel, pool->pages, &bytes));
-  fork_plan_kernel<<<1, PLAN_THREADS, bytes, s>>>(*pool, parent, status);
-  CUDA_TRY(cudaGetLastError());
+  B200Q_TRY(launch_dependent(fork_plan_kernel, dim3(1), dim3(PLAN_THREADS), bytes, s, *pool, parent, status));
   // 32 columns a tile where they fit, at least 8
   int columns = FORK_TILE / pool->sequences;
   columns = columns > 32 ? 32 : columns;
   const int tiles = ceil_div(pool->table_width, columns), table_blocks = tiles < sms ? tiles : sms;
   const int64_t copies = (int64_t)pool->sequences * 2 * cache->layers;
   const int copy_blocks = (int)(copies < 4 * sms ? copies : 4 * sms);
-  cudaLaunchAttribute attr;
-  cudaLaunchConfig_t cfg = launch_config(dim3(table_blocks + copy_blocks), dim3(FORK_THREADS), 0, s, &attr, true);
-  CUDA_TRY(cudaLaunchKernelEx(&cfg, fork_kernel, *cache, *pool, parent, table_blocks, columns));
-  return B200Q_OK;
+  return launch_dependent(fork_kernel, dim3(table_blocks + copy_blocks), dim3(FORK_THREADS), 0, s, *cache, *pool, parent, table_blocks, columns);
 }
 
 int b200q_kv_compact_dev(const b200q_kv_cache* cache, const b200q_kv_pool* pool, const int32_t* path, int64_t path_stride,
@@ -494,14 +490,9 @@ int b200q_kv_compact_dev(const b200q_kv_cache* cache, const b200q_kv_pool* pool,
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   // (a block with nothing to move is gone in a microsecond: the grid only has to keep the memory busy)
   const int64_t items = (int64_t)pool->sequences * 2 * cache->layers;
-  compact_kernel<<<(unsigned)(items < 65536 ? items : 65536), COMPACT_THREADS, 0, s>>>(*cache, *pool, path, path_stride, path_width, path_length,
-                                                                                       in_place ? pool->scratch : length_out);
-  CUDA_TRY(cudaGetLastError());
-  if (in_place) {
-    cudaLaunchAttribute attr;
-    cudaLaunchConfig_t cfg = launch_config(dim3(1), dim3(KV_MAX_SEQUENCES), 0, s, &attr, true);
-    CUDA_TRY(cudaLaunchKernelEx(&cfg, lengths_kernel, (const int32_t*)pool->scratch, pool->length, pool->sequences));
-  }
+  B200Q_TRY(launch_dependent(compact_kernel, dim3((unsigned)(items < 65536 ? items : 65536)), dim3(COMPACT_THREADS), 0, s, *cache, *pool, path,
+                             path_stride, path_width, path_length, in_place ? pool->scratch : length_out));
+  if (in_place) B200Q_TRY(launch_dependent(lengths_kernel, dim3(1), dim3(KV_MAX_SEQUENCES), 0, s, pool->scratch, pool->length, pool->sequences));
   return B200Q_OK;
 }
 

@@ -53,6 +53,7 @@ __global__ void __launch_bounds__(ROPE_THREADS) rope_kernel(const __grid_constan
   const int rows = (int)(io.rows - r0 < a.rows_per_block ? io.rows - r0 : a.rows_per_block);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   ptx::griddep_launch_dependents();
+  ptx::griddep_wait();
 
   if (warp < rows) {
     const int64_t r = r0 + warp;
@@ -189,7 +190,7 @@ int launch_rope(RopeArgs& a, bool f16, bool wide, int sms, cudaStream_t s) {
   if (blocks > 0x7fffffffLL) return set_error(B200Q_ERR_UNSUPPORTED, "rope: too many rows");
   const dim3 grid((unsigned)blocks, (a.heads + a.heads_per_block - 1) / a.heads_per_block);
   const size_t smem = (size_t)rows * half * sizeof(float2);
-#define B200Q_ROPE(F, I, W) rope_kernel<F, I, W><<<grid, ROPE_THREADS, smem, s>>>(a)
+#define B200Q_ROPE(F, I, W) return launch_dependent(rope_kernel<F, I, W>, grid, dim3(ROPE_THREADS), smem, s, a)
   if (f16) {
     if (interleaved) { if (wide) B200Q_ROPE(true, true, true); else B200Q_ROPE(true, true, false); }
     else { if (wide) B200Q_ROPE(true, false, true); else B200Q_ROPE(true, false, false); }
@@ -198,8 +199,6 @@ int launch_rope(RopeArgs& a, bool f16, bool wide, int sms, cudaStream_t s) {
     else { if (wide) B200Q_ROPE(false, false, true); else B200Q_ROPE(false, false, false); }
   }
 #undef B200Q_ROPE
-  CUDA_TRY(cudaGetLastError());
-  return B200Q_OK;
 }
 
 bool aligned16(const void* p, int64_t row_stride, int64_t head_stride) {

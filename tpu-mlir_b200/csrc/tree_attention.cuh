@@ -1,0 +1,307 @@
+// What the two kernels of the attention over the paged cache share: the line of units and its runs, masks, the loading warp.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "kv_cache.h"
+#include "ptx_sm100.cuh"
+
+namespace b200q {
+namespace attn {
+
+constexpr int UNIT = 64;   // positions of a unit
+
+struct AttnArgs {
+  b200q_kv_cache cache;
+  b200q_kv_pool pool;
+  b200q_tree_attention io;
+  int group;          // query heads of a cache head
+  float scale_log2;   // scale * log2(e)
+  int box;            // rows of a TMA box
+  int min_run;        // the shortest run of the line that a block takes, if there is so much
+  unsigned long long wait_ns;   // no wait inside the kernel lasts longer
+  int expect_extra;             // test aid: bytes that a stage waits for and that never come (0 in normal use)
+  float* partial;     // [blocks][2][rows of a tile][dim + 4]: sums, maximum (log2 domain), total, nothing
+  struct SplitItem* items;   // [blocks]
+};
+
+// The item that starts in a block's run and ends in a later one's.
+struct SplitItem {
+  int parts;       // blocks that hold a part of it; 0: none
+  int first_row;   // of its sequence
+  int row0, rows;  // its tile's first (node, head of the group) and how many the sequence has
+  int head;        // cache head
+};
+
+struct Sequence {
+  int first_row, nodes, length, total;   // total: committed positions and nodes
+};
+__device__ __forceinline__ Sequence load_sequence(const AttnArgs& a, int s) {
+  Sequence q;
+  const int64_t b = a.io.row_start[s], e = a.io.row_start[s + 1];
+  const int64_t end = e < a.io.rows ? e : a.io.rows;
+  q.first_row = (int)b;
+  q.nodes = b >= 0 && end > b ? (int)(end - b) : 0;
+  q.length = kv_length(a.pool, s);
+  const int64_t most = (int64_t)a.pool.table_width * a.pool.page_size, all = (int64_t)q.length + q.nodes;
+  q.total = (int)(all < most ? all : most);
+  return q;
+}
+
+// a box of a page's rows: x byte of the head, y slot, z head, w page; what lies outside becomes zeros
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z, int w) {
+  asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
+               "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z), "r"(w)
+               : "memory");
+}
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+template <bool F16>
+__device__ __forceinline__ uint32_t pack_pair(float lo, float hi) {
+  if (F16) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+// a 16-bit number that is infinite or NaN
+template <bool F16>
+__device__ __forceinline__ bool not_finite(uint32_t bits) {
+  constexpr uint32_t E = F16 ? 0x7c00u : 0x7f80u;
+  return (bits & E) == E;
+}
+template <bool F16>
+__device__ __forceinline__ float from_bits(uint32_t bits) {
+  return F16 ? __half2float(__ushort_as_half((unsigned short)bits)) : __uint_as_float(bits << 16);
+}
+__device__ __forceinline__ uint64_t low_bits(int n) { return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1; }
+
+// Which of the 64 positions from `p0` on node `node` sees: all committed ones, and the nodes that its mask names (a chain: up to
+// itself).
+__device__ __forceinline__ uint64_t sees(const AttnArgs& a, int row, int node, int length, int p0) {
+  const int base = p0 - length;   // node at the first position, negative: committed
+  if (base <= -64) return ~0ull;
+  if (!a.io.mask) return low_bits(node - base + 1);
+  const uint32_t* mask = a.io.mask + (int64_t)row * a.io.mask_stride;
+  const int from = base > 0 ? base : 0;
+  const int64_t w = from >> 5;
+  const int sh = from & 31;
+  const uint64_t w0 = w < a.io.mask_stride ? mask[w] : 0u, w1 = w + 1 < a.io.mask_stride ? mask[w + 1] : 0u,
+                 w2 = w + 2 < a.io.mask_stride ? mask[w + 2] : 0u;
+  uint64_t bits = (w0 | w1 << 32) >> sh;
+  if (sh) bits |= w2 << (64 - sh);
+  return base >= 0 ? bits : low_bits(-base) | bits << -base;
+}
+
+// ---- the line of units: which unit stands at a position of it
+struct Line {
+  const Sequence* seqs;
+  int sequences, heads, group, tile_rows;
+};
+// An item (sequence, cache head, row tile) takes ITEM_COST positions of the line and one for each unit: what a block spends on an
+// item besides its units (queries, the sums' way out) counts when runs are made equal.
+constexpr int ITEM_COST = 2;
+struct Place {
+  long long pos;                     // in the line
+  int s, head, tile, unit;           // row tile of the sequence, unit of the item
+  int tiles, units, total, length, nodes, first_row;
+  __device__ __forceinline__ void enter(const Line& line, int seq) {
+    const Sequence q = line.seqs[seq];
+    s = seq;
+    tiles = (int)(((long long)q.nodes * line.group + line.tile_rows - 1) / line.tile_rows);
+    units = (q.total + UNIT - 1) / UNIT;
+    total = q.total;
+    length = q.length;
+    nodes = q.nodes;
+    first_row = q.first_row;
+  }
+  // the unit at `pos` or the first one after it; sums: the line's length up to and with each sequence
+  __device__ __forceinline__ void find(const Line& line, const long long* sums, long long at) {
+    int lo = 0, hi = line.sequences - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (sums[mid] > at) hi = mid;
+      else lo = mid + 1;
+    }
+    enter(line, lo);
+    const long long local = at - (lo ? sums[lo - 1] : 0), item = local / (units + ITEM_COST);
+    const int in = (int)(local - item * (units + ITEM_COST)) - ITEM_COST;
+    head = (int)(item / tiles);
+    tile = (int)(item - (long long)head * tiles);
+    unit = in > 0 ? in : 0;
+    pos = at + (in < 0 ? -in : 0);
+  }
+  // row tiles of a head stand next to each other: they read the same keys
+  __device__ __forceinline__ void next(const Line& line) {
+    ++pos;
+    if (++unit < units) return;
+    unit = 0;
+    pos += ITEM_COST;
+    if (++tile < tiles) return;
+    tile = 0;
+    if (++head < line.heads) return;
+    head = 0;
+    int q = s + 1;
+    while (q < line.sequences && line.seqs[q].nodes == 0) ++q;
+    if (q < line.sequences) enter(line, q);
+  }
+};
+
+// Fills seqs and sums (the line's length up to and with each sequence) for all threads of the block; returns the line's length.
+template <int THREADS>
+__device__ __forceinline__ long long lay_out(const AttnArgs& a, int tile_rows, Sequence* seqs, long long* sums, long long* buf) {
+  const int n = a.pool.sequences, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int each = (n + THREADS - 1) / THREADS;
+  long long mine = 0;
+  for (int i = 0; i < each; ++i) {
+    const int s = tid * each + i;
+    if (s >= n) break;
+    const Sequence q = load_sequence(a, s);
+    const long long tiles = ((long long)q.nodes * a.group + tile_rows - 1) / tile_rows;
+    mine += a.cache.heads * tiles * ((q.total + UNIT - 1) / UNIT + ITEM_COST);
+    seqs[s] = q;
+    sums[s] = mine;
+  }
+  long long upto = mine;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const long long o = __shfl_up_sync(0xffffffffu, upto, d);
+    if (lane >= d) upto += o;
+  }
+  if (lane == 31) buf[warp] = upto;
+  __syncthreads();
+  long long before = upto - mine, total = 0;
+#pragma unroll
+  for (int w = 0; w < THREADS / 32; ++w) {
+    if (w < warp) before += buf[w];
+    total += buf[w];
+  }
+  for (int i = 0; i < each; ++i)
+    if (tid * each + i < n) sums[tid * each + i] += before;
+  __syncthreads();
+  return total;
+}
+
+// ---- loading.  Layout of a tile: [64 elements of the head][row][128 bytes], 16-byte pieces swizzled by the row.
+__device__ __forceinline__ uint32_t tile_at(int row, int piece) {
+  return (piece >> 3) * (UNIT * 128) + row * 128 + (((piece & 7) ^ (row & 7)) * 16);
+}
+// Keys and values travel in rings of their own: the computing side is done with a unit's keys before its values.
+template <int KEYS, int VALUES>
+struct Rings {
+  static constexpr int NOTES = 8;   // units whose `there` is kept: more than any role is behind the loads
+  uint64_t k_full[KEYS], k_empty[KEYS], v_full[VALUES], v_empty[VALUES];
+  // which rows of a unit are positions of the sequence in a page of the pool (the others are zeros, or whatever a page holds past the
+  // sequence's end)
+  uint64_t there[NOTES];
+  static_assert(KEYS + 2 < NOTES && VALUES + 2 < NOTES, "");
+  __device__ __forceinline__ void init(int readers) {
+    for (int i = 0; i < KEYS; ++i) {
+      ptx::mbar_init(ptx::smem_u32(&k_full[i]), 1);
+      ptx::mbar_init(ptx::smem_u32(&k_empty[i]), readers);
+    }
+    for (int i = 0; i < VALUES; ++i) {
+      ptx::mbar_init(ptx::smem_u32(&v_full[i]), 1);
+      ptx::mbar_init(ptx::smem_u32(&v_empty[i]), readers);
+    }
+  }
+};
+// a place in a ring, and the parity of the phase that is waited for there
+template <int N>
+struct Slot {
+  int i = 0;
+  uint32_t phase;
+  __device__ __forceinline__ explicit Slot(uint32_t p) : phase(p) {}
+  __device__ __forceinline__ void next() {
+    if (++i == N) {
+      i = 0;
+      phase ^= 1;
+    }
+  }
+};
+
+// The loading warp's life: every unit of the block's run into the rings.  A box is `box` rows (the greatest common divisor of a page's
+// and a unit's, so no box is cut by either) of 64 elements.
+template <int DIM, int KEYS, int VALUES, typename Wait>
+__device__ __forceinline__ void load_units(const AttnArgs& a, const CUtensorMap* km, const CUtensorMap* vm, const Line& line, Place at, long long end,
+                                           uint32_t k_ring, uint32_t v_ring, Rings<KEYS, VALUES>& r, Wait wait) {
+  constexpr int TILE = UNIT * DIM * 2, HALVES = DIM / 64;
+  const int lane = threadIdx.x & 31, box = a.box, boxes = UNIT / box, page_size = a.pool.page_size;
+  Slot<KEYS> ks(1);     // the first pass over a ring finds it empty
+  Slot<VALUES> vs(1);
+  uint32_t k_sent = 0, v_sent = 0;
+  // the place of box `lane` (and lane + 32) of the unit that `at` stands at: page (-1: none) and slot of its first row
+  int page[2], slot[2], rows;
+  auto look_up = [&]() {
+    rows = at.total - at.unit * UNIT;   // may be more than a unit's
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int b = lane + 32 * j, pos = at.unit * UNIT + b * box;
+      page[j] = -1;
+      slot[j] = 0;
+      if (b < boxes && pos < at.total) {
+        page[j] = kv_page(a.pool, at.s, pos);
+        slot[j] = (int)((unsigned)pos % (unsigned)page_size);
+      }
+    }
+  };
+  look_up();
+  while (at.pos < end) {
+    const int head = at.head, pg0 = page[0], pg1 = page[1], sl0 = slot[0], sl1 = slot[1], here = rows;
+    at.next(line);
+    if (at.pos < end) look_up();   // the next unit's entries are on their way while this one's boxes go out
+    uint64_t in = 0;
+    if (pg0 >= 0) in |= low_bits(box) << (lane * box);
+    if (pg1 >= 0) in |= low_bits(box) << ((lane + 32) * box);
+    in = (uint64_t)__reduce_or_sync(0xffffffffu, (uint32_t)(in >> 32)) << 32 | __reduce_or_sync(0xffffffffu, (uint32_t)in);
+    // a copy a lane: box, then which 64 elements
+    auto send = [&](const CUtensorMap* map, uint32_t dst, uint32_t bar) {
+      for (int i = lane; i - lane < boxes * HALVES; i += 32) {
+        const int b = i / HALVES, x = i % HALVES;
+        const int p0 = __shfl_sync(0xffffffffu, pg0, b & 31), p1 = __shfl_sync(0xffffffffu, pg1, b & 31);
+        const int s0 = __shfl_sync(0xffffffffu, sl0, b & 31), s1 = __shfl_sync(0xffffffffu, sl1, b & 31);
+        if (b < boxes) {
+          const int pg = b < 32 ? p0 : p1, sl = b < 32 ? s0 : s1;
+          tma_load_4d(dst + x * (UNIT * 128) + b * box * 128, map, bar, x * 128, sl, head, pg < 0 ? a.pool.pages : pg);
+        }
+      }
+    };
+    if (!wait(&r.k_empty[ks.i], ks.phase, 1)) break;
+    uint32_t bar = ptx::smem_u32(&r.k_full[ks.i]);
+    if (lane == 0) {
+      r.there[k_sent % r.NOTES] = in & low_bits(here);
+      ptx::mbar_arrive_expect_tx(bar, TILE + a.expect_extra);
+    }
+    __syncwarp();
+    send(km, k_ring + ks.i * TILE, bar);
+    ++k_sent;
+    ks.next();
+    if (!wait(&r.v_empty[vs.i], vs.phase, 2)) break;
+    bar = ptx::smem_u32(&r.v_full[vs.i]);
+    if (lane == 0) ptx::mbar_arrive_expect_tx(bar, TILE + a.expect_extra);
+    __syncwarp();
+    send(vm, v_ring + vs.i * TILE, bar);
+    ++v_sent;
+    vs.next();
+  }
+  // what is still on its way (when a wait ran out somewhere) lands before the block is gone
+  int flag = 0;
+  for (uint32_t i = 0; i < KEYS; ++i)
+    if (i < k_sent) ptx::mbar_wait_bounded(ptx::smem_u32(&r.k_full[i]), ((k_sent - i - 1) / KEYS) & 1, &flag, 1, a.wait_ns);
+  for (uint32_t i = 0; i < VALUES; ++i)
+    if (i < v_sent) ptx::mbar_wait_bounded(ptx::smem_u32(&r.v_full[i]), ((v_sent - i - 1) / VALUES) & 1, &flag, 1, a.wait_ns);
+  __syncwarp();
+}
+
+// Launchers: the kernel on mma.sync (tree_attention.cu) and the one on tcgen05 (tree_attention_umma.cu), each followed by the join.
+int make_map(CUtensorMap* map, const AttnArgs& a, const void* base);
+int launch_join(const AttnArgs& a, int blocks, int tile_rows, int dim, cudaStream_t s);
+constexpr int UMMA_ROWS = 128;
+int launch_umma(const AttnArgs& a, int sms, cudaStream_t s);
+
+}  // namespace attn
+}  // namespace b200q
