@@ -86,7 +86,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap km, const __grid_const
   uint8_t* smem = smem_raw + (-ptx::smem_u32(smem_raw) & 1023);   // the swizzle goes by the address
   __shared__ long long scan_buf[BLOCK / 32];
   __shared__ uint32_t bad[2];                    // rows of the unit whose values hold infinities or NaN
-  __shared__ Rings<STAGES, STAGES> rings;
+  __shared__ Ring<STAGES> ring;
   __shared__ int abort_flag;
   float* merge = reinterpret_cast<float*>(smem + STAGES * 2 * S::TILE);
   float* merge_ml = merge + S::ROWS * 64;
@@ -97,7 +97,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap km, const __grid_const
   ptx::griddep_launch_dependents();
 
   if (tid == 0) {
-    rings.init(COMPUTERS / 32);
+    ring.init(COMPUTERS / 32);
     ptx::fence_barrier_init();
     abort_flag = 0;
     bad[0] = bad[1] = 0;
@@ -128,7 +128,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap km, const __grid_const
 
   if (warp >= COMPUTERS / 32) {
     // ---------------------------------------------------------------- loading
-    load_units<DIM>(a, &km, &vm, line, at, u1, smem_base, smem_base + STAGES * S::TILE, rings, wait);
+    load_units<DIM>(a, &km, &vm, line, at, u1, smem_base, ring, wait);
     if (dead && lane == 0 && a.io.status) atomicMax(a.io.status, abort_flag);
     return;
   }
@@ -170,11 +170,11 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap km, const __grid_const
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[k][e] = 0.f;
     }
-    wait(&rings.k_full[slot.i], slot.phase, 3);
+    wait(&ring.full[slot.i], slot.phase, 3);
 
     // ---- scores of 16 rows x COLS positions
     // (pieces 2k and 2k + 1 of a row: the swizzle makes the step from k to k + 1 an exclusive or of 32 bytes)
-    const uint32_t ks = smem_base + slot.i * S::TILE, vs = ks + STAGES * S::TILE;
+    const uint32_t ks = smem_base + slot.i * 2 * S::TILE, vs = ks + S::TILE;
     const uint32_t k_lane = ks + tile_at(wc * S::COLS + (lane >> 4) * 8 + (lane & 7), (lane >> 3) & 1);
     const uint32_t v_lane = vs + tile_at(wc * S::COLS + ((lane >> 3) & 1) * 8 + (lane & 7), lane >> 4);
     float sc[NT][4];
@@ -195,12 +195,9 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap km, const __grid_const
       }
     }
 
-    __syncwarp();
-    if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&rings.k_empty[slot.i]));
-
     // ---- what is not seen
     const int p0 = at.unit * UNIT;
-    const uint64_t in_pool = rings.there[count++ % rings.NOTES];
+    const uint64_t in_pool = ring.there[count++ % ring.NOTES];
     const bool drafted = p0 + UNIT > at.length;
     uint64_t see[2] = {~0ull, ~0ull};
     bool fix = false;
@@ -216,7 +213,6 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap km, const __grid_const
             if (!(mine64 >> (t * 8 + e) & 1)) sc[t][2 * h + e] = -INFINITY;
       }
       if (drafted) {
-        wait(&rings.v_full[slot.i], slot.phase, 4);
         // Values of drafted nodes meet weights of zero in rows that do not see them: infinite or NaN ones are taken out of the
         // tile (and added below where they are seen), or they would make those rows NaN.
         bool found = false;
@@ -271,7 +267,6 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap km, const __grid_const
       }
     }
 
-    wait(&rings.v_full[slot.i], slot.phase, 4);
     // ---- weights (rounded to the 16-bit type: the tensor cores take no wider pair; the rounding is unbiased and averages out
     // over positions) times values
 #pragma unroll
@@ -326,7 +321,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap km, const __grid_const
       computers_sync();
     }
     __syncwarp();
-    if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&rings.v_empty[slot.i]));
+    if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&ring.empty[slot.i]));
     slot.next();
 
     // ---- the end of the item, or of this block's part
@@ -493,7 +488,7 @@ int launch_rows(const AttnArgs& a, int sms, cudaStream_t s) {
   const int64_t rows = (a.io.rows + a.pool.sequences - 1) / a.pool.sequences * a.group;
   if (rows <= 16) return launch<F16, DIM, 1, 4>(a, sms, s);
   if (rows <= 32 || DIM > 128) return launch<F16, DIM, 2, 2>(a, sms, s);
-  return launch_umma(a, sms, s);
+  return launch_umma(a, rows > UMMA_ROWS, sms, s);
 }
 
 template <bool F16>

@@ -135,10 +135,11 @@ struct Place {
     unit = in > 0 ? in : 0;
     pos = at + (in < 0 ? -in : 0);
   }
-  // row tiles of a head stand next to each other: they read the same keys
-  __device__ __forceinline__ void next(const Line& line) {
-    ++pos;
-    if (++unit < units) return;
+  __device__ __forceinline__ void next(const Line& line) { skip(line, 1); }
+  // past `count` units of the item, no more than it has left.  Row tiles of a head stand next to each other: they read the same keys
+  __device__ __forceinline__ void skip(const Line& line, int count) {
+    pos += count;
+    if ((unit += count) < units) return;
     unit = 0;
     pos += ITEM_COST;
     if (++tile < tiles) return;
@@ -190,23 +191,18 @@ __device__ __forceinline__ long long lay_out(const AttnArgs& a, int tile_rows, S
 __device__ __forceinline__ uint32_t tile_at(int row, int piece) {
   return (piece >> 3) * (UNIT * 128) + row * 128 + (((piece & 7) ^ (row & 7)) * 16);
 }
-// Keys and values travel in rings of their own: the computing side is done with a unit's keys before its values.
-template <int KEYS, int VALUES>
-struct Rings {
-  static constexpr int NOTES = 8;   // units whose `there` is kept: more than any role is behind the loads
-  uint64_t k_full[KEYS], k_empty[KEYS], v_full[VALUES], v_empty[VALUES];
+template <int STAGES>
+struct Ring {
+  static constexpr int NOTES = 16;   // units whose `there` is kept: more than any role is behind the loads
+  uint64_t full[STAGES], empty[STAGES];
   // which rows of a unit are positions of the sequence in a page of the pool (the others are zeros, or whatever a page holds past the
   // sequence's end)
   uint64_t there[NOTES];
-  static_assert(KEYS + 2 < NOTES && VALUES + 2 < NOTES, "");
+  static_assert(STAGES + 4 < NOTES, "");
   __device__ __forceinline__ void init(int readers) {
-    for (int i = 0; i < KEYS; ++i) {
-      ptx::mbar_init(ptx::smem_u32(&k_full[i]), 1);
-      ptx::mbar_init(ptx::smem_u32(&k_empty[i]), readers);
-    }
-    for (int i = 0; i < VALUES; ++i) {
-      ptx::mbar_init(ptx::smem_u32(&v_full[i]), 1);
-      ptx::mbar_init(ptx::smem_u32(&v_empty[i]), readers);
+    for (int i = 0; i < STAGES; ++i) {
+      ptx::mbar_init(ptx::smem_u32(&full[i]), 1);
+      ptx::mbar_init(ptx::smem_u32(&empty[i]), readers);
     }
   }
 };
@@ -224,16 +220,15 @@ struct Slot {
   }
 };
 
-// The loading warp's life: every unit of the block's run into the rings.  A box is `box` rows (the greatest common divisor of a page's
-// and a unit's, so no box is cut by either) of 64 elements.
-template <int DIM, int KEYS, int VALUES, typename Wait>
+// The loading warp's life: every unit of the block's run into the ring, keys and values of a stage one after the other.  A box is `box`
+// rows (the greatest common divisor of a page's and a unit's, so no box is cut by either) of 64 elements.
+template <int DIM, int STAGES, typename Wait>
 __device__ __forceinline__ void load_units(const AttnArgs& a, const CUtensorMap* km, const CUtensorMap* vm, const Line& line, Place at, long long end,
-                                           uint32_t k_ring, uint32_t v_ring, Rings<KEYS, VALUES>& r, Wait wait) {
-  constexpr int TILE = UNIT * DIM * 2, HALVES = DIM / 64;
+                                           uint32_t stages, Ring<STAGES>& ring, Wait wait) {
+  constexpr int TILE = UNIT * DIM * 2, PARTS = 2 * (DIM / 64);
   const int lane = threadIdx.x & 31, box = a.box, boxes = UNIT / box, page_size = a.pool.page_size;
-  Slot<KEYS> ks(1);     // the first pass over a ring finds it empty
-  Slot<VALUES> vs(1);
-  uint32_t k_sent = 0, v_sent = 0;
+  Slot<STAGES> at_stage(1);     // the first pass over the ring finds it empty
+  uint32_t sent = 0;
   // the place of box `lane` (and lane + 32) of the unit that `at` stands at: page (-1: none) and slot of its first row
   int page[2], slot[2], rows;
   auto look_up = [&]() {
@@ -258,42 +253,30 @@ __device__ __forceinline__ void load_units(const AttnArgs& a, const CUtensorMap*
     if (pg0 >= 0) in |= low_bits(box) << (lane * box);
     if (pg1 >= 0) in |= low_bits(box) << ((lane + 32) * box);
     in = (uint64_t)__reduce_or_sync(0xffffffffu, (uint32_t)(in >> 32)) << 32 | __reduce_or_sync(0xffffffffu, (uint32_t)in);
-    // a copy a lane: box, then which 64 elements
-    auto send = [&](const CUtensorMap* map, uint32_t dst, uint32_t bar) {
-      for (int i = lane; i - lane < boxes * HALVES; i += 32) {
-        const int b = i / HALVES, x = i % HALVES;
-        const int p0 = __shfl_sync(0xffffffffu, pg0, b & 31), p1 = __shfl_sync(0xffffffffu, pg1, b & 31);
-        const int s0 = __shfl_sync(0xffffffffu, sl0, b & 31), s1 = __shfl_sync(0xffffffffu, sl1, b & 31);
-        if (b < boxes) {
-          const int pg = b < 32 ? p0 : p1, sl = b < 32 ? s0 : s1;
-          tma_load_4d(dst + x * (UNIT * 128) + b * box * 128, map, bar, x * 128, sl, head, pg < 0 ? a.pool.pages : pg);
-        }
-      }
-    };
-    if (!wait(&r.k_empty[ks.i], ks.phase, 1)) break;
-    uint32_t bar = ptx::smem_u32(&r.k_full[ks.i]);
+    if (!wait(&ring.empty[at_stage.i], at_stage.phase, 1)) break;
+    const uint32_t bar = ptx::smem_u32(&ring.full[at_stage.i]), dst = stages + at_stage.i * 2 * TILE;
     if (lane == 0) {
-      r.there[k_sent % r.NOTES] = in & low_bits(here);
-      ptx::mbar_arrive_expect_tx(bar, TILE + a.expect_extra);
+      ring.there[sent % ring.NOTES] = in & low_bits(here);
+      ptx::mbar_arrive_expect_tx(bar, 2 * TILE + a.expect_extra);
     }
     __syncwarp();
-    send(km, k_ring + ks.i * TILE, bar);
-    ++k_sent;
-    ks.next();
-    if (!wait(&r.v_empty[vs.i], vs.phase, 2)) break;
-    bar = ptx::smem_u32(&r.v_full[vs.i]);
-    if (lane == 0) ptx::mbar_arrive_expect_tx(bar, TILE + a.expect_extra);
-    __syncwarp();
-    send(vm, v_ring + vs.i * TILE, bar);
-    ++v_sent;
-    vs.next();
+    // a copy a lane: keys before values, then box, then which 64 elements
+    for (int i = lane; i - lane < boxes * PARTS; i += 32) {
+      const int v = i >= boxes * (PARTS / 2), k = i - v * boxes * (PARTS / 2), b = k / (PARTS / 2), x = k % (PARTS / 2);
+      const int p0 = __shfl_sync(0xffffffffu, pg0, b & 31), p1 = __shfl_sync(0xffffffffu, pg1, b & 31);
+      const int s0 = __shfl_sync(0xffffffffu, sl0, b & 31), s1 = __shfl_sync(0xffffffffu, sl1, b & 31);
+      if (i < boxes * PARTS) {
+        const int pg = b < 32 ? p0 : p1, sl = b < 32 ? s0 : s1;
+        tma_load_4d(dst + v * TILE + x * (UNIT * 128) + b * box * 128, v ? vm : km, bar, x * 128, sl, head, pg < 0 ? a.pool.pages : pg);
+      }
+    }
+    ++sent;
+    at_stage.next();
   }
   // what is still on its way (when a wait ran out somewhere) lands before the block is gone
   int flag = 0;
-  for (uint32_t i = 0; i < KEYS; ++i)
-    if (i < k_sent) ptx::mbar_wait_bounded(ptx::smem_u32(&r.k_full[i]), ((k_sent - i - 1) / KEYS) & 1, &flag, 1, a.wait_ns);
-  for (uint32_t i = 0; i < VALUES; ++i)
-    if (i < v_sent) ptx::mbar_wait_bounded(ptx::smem_u32(&r.v_full[i]), ((v_sent - i - 1) / VALUES) & 1, &flag, 1, a.wait_ns);
+  for (uint32_t i = 0; i < STAGES; ++i)
+    if (i < sent) ptx::mbar_wait_bounded(ptx::smem_u32(&ring.full[i]), ((sent - i - 1) / STAGES) & 1, &flag, 1, a.wait_ns);
   __syncwarp();
 }
 
@@ -301,7 +284,7 @@ __device__ __forceinline__ void load_units(const AttnArgs& a, const CUtensorMap*
 int make_map(CUtensorMap* map, const AttnArgs& a, const void* base);
 int launch_join(const AttnArgs& a, int blocks, int tile_rows, int dim, cudaStream_t s);
 constexpr int UMMA_ROWS = 128;
-int launch_umma(const AttnArgs& a, int sms, cudaStream_t s);
+int launch_umma(const AttnArgs& a, bool pair, int sms, cudaStream_t s);   // pair: two row tiles at a time
 
 }  // namespace attn
 }  // namespace b200q
