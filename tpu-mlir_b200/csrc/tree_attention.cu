@@ -47,7 +47,7 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-constexpr int COMPUTERS = 128, BLOCK = COMPUTERS + 32;
+constexpr int COMPUTERS = 128, BLOCK = COMPUTERS + 32 * LOADERS;
 
 __device__ __forceinline__ void computers_sync() { asm volatile("barrier.cta.sync 1, 128;" ::: "memory"); }
 __device__ __forceinline__ bool computers_or(bool x) {
@@ -118,17 +118,14 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap km, const __grid_const
   const uint16_t* vp = static_cast<const uint16_t*>(a.cache.v) + a.io.layer * a.cache.layer_stride;
   const uint32_t smem_base = ptx::smem_u32(smem);
   // A wait that runs out (it cannot, short of a fault) ends all waiting: the roles go on without (or stop, where they would load), so
-  // that no barrier is left short, and the status says so.  A warp agrees on it.
+  // that no barrier is left short, and the status says so.
   bool dead = false;
-  auto wait = [&](uint64_t* bar, uint32_t parity, int where) {
-    const bool here = !dead && ptx::mbar_wait_bounded(ptx::smem_u32(bar), parity, &abort_flag, where, a.wait_ns);
-    dead = !__all_sync(0xffffffffu, here);
-    return !dead;
-  };
+  auto wait = [&](uint64_t* bar, uint32_t parity, int where) { return warp_wait(bar, parity, dead, &abort_flag, where, a.wait_ns); };
 
   if (warp >= COMPUTERS / 32) {
     // ---------------------------------------------------------------- loading
-    load_units<DIM>(a, &km, &vm, line, at, u1, smem_base, ring, wait);
+    if (warp == COMPUTERS / 32) load_units<DIM>(a, &km, line, at, u1, smem_base, ring, 0, wait);
+    else load_units<DIM>(a, &vm, line, at, u1, smem_base, ring, 1, wait);
     if (dead && lane == 0 && a.io.status) atomicMax(a.io.status, abort_flag);
     return;
   }

@@ -48,11 +48,17 @@ __device__ __forceinline__ Sequence load_sequence(const AttnArgs& a, int s) {
   return q;
 }
 
-// a box of a page's rows: x byte of the head, y slot, z head, w page; what lies outside becomes zeros
+// A box of a page's rows: x byte of the head, y slot, z head, w page; what lies outside becomes zeros.  Called by a whole warp with
+// the same arguments, issued by one elected thread (a copy from a branch, or one a lane, took 100 clocks each).
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z, int w) {
-  asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
-               "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z), "r"(w)
-               : "memory");
+  asm volatile(
+      "{\n\t"
+      ".reg .pred one;\n\t"
+      "elect.sync _|one, 0xffffffff;\n\t"
+      "@one cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];\n\t"
+      "}\n" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z), "r"(w)
+      : "memory");
 }
 __device__ __forceinline__ float exp2_approx(float x) {
   float y;
@@ -191,6 +197,7 @@ __device__ __forceinline__ long long lay_out(const AttnArgs& a, int tile_rows, S
 __device__ __forceinline__ uint32_t tile_at(int row, int piece) {
   return (piece >> 3) * (UNIT * 128) + row * 128 + (((piece & 7) ^ (row & 7)) * 16);
 }
+constexpr int LOADERS = 2;   // warps: one for keys, one for values
 template <int STAGES>
 struct Ring {
   static constexpr int NOTES = 16;   // units whose `there` is kept: more than any role is behind the loads
@@ -201,7 +208,7 @@ struct Ring {
   static_assert(STAGES + 4 < NOTES, "");
   __device__ __forceinline__ void init(int readers) {
     for (int i = 0; i < STAGES; ++i) {
-      ptx::mbar_init(ptx::smem_u32(&full[i]), 1);
+      ptx::mbar_init(ptx::smem_u32(&full[i]), LOADERS);
       ptx::mbar_init(ptx::smem_u32(&empty[i]), readers);
     }
   }
@@ -220,58 +227,100 @@ struct Slot {
   }
 };
 
-// The loading warp's life: every unit of the block's run into the ring, keys and values of a stage one after the other.  A box is `box`
-// rows (the greatest common divisor of a page's and a unit's, so no box is cut by either) of 64 elements.
+// A warp's wait for a barrier; false once any wait of the block has run out (dead: this warp's memory of that).  The first look costs 40
+// clocks when the phase is over; going through the bounded loop for it, 100 to 170.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, bool& dead, int* abort_flag, int where, unsigned long long ns) {
+  const uint32_t b = ptx::smem_u32(bar);
+  if (__all_sync(0xffffffffu, ptx::mbar_try_wait(b, parity))) return !dead;
+  const bool here = !dead && ptx::mbar_wait_bounded_fast<20>(b, parity, abort_flag, where, ns);
+  dead = !__all_sync(0xffffffffu, here);
+  return !dead;
+}
+
+// A loading warp's life: the keys (which 0) or the values (1) of every unit of the block's run into the ring.  A box is `box` rows (the
+// greatest common divisor of a page's and a unit's, so no box is cut by either) of 64 elements.  A lane looks up one box: 32 lanes
+// serve the next 32 * box / 64 units at once, a group ahead of their copies, or the table's latency (700 clocks) would be paid for
+// every unit.  (With boxes of one row a unit has 64: a lane looks up two.)  Issuing a copy takes 95 clocks, which is why there are two
+// such warps: sixteen copies, what a unit of pages of 16 slots takes, are 1530.
 template <int DIM, int STAGES, typename Wait>
-__device__ __forceinline__ void load_units(const AttnArgs& a, const CUtensorMap* km, const CUtensorMap* vm, const Line& line, Place at, long long end,
-                                           uint32_t stages, Ring<STAGES>& ring, Wait wait) {
-  constexpr int TILE = UNIT * DIM * 2, PARTS = 2 * (DIM / 64);
+__device__ __forceinline__ void load_units(const AttnArgs& a, const CUtensorMap* map, const Line& line, Place at, long long end,
+                                           uint32_t stages, Ring<STAGES>& ring, int which, Wait wait) {
+  constexpr int TILE = UNIT * DIM * 2, PARTS = DIM / 64;
   const int lane = threadIdx.x & 31, box = a.box, boxes = UNIT / box, page_size = a.pool.page_size;
+  const int group = boxes < 32 ? 32 / boxes : 1, box0 = lane % boxes;   // units of a group; this lane's box of its unit
   Slot<STAGES> at_stage(1);     // the first pass over the ring finds it empty
   uint32_t sent = 0;
-  // the place of box `lane` (and lane + 32) of the unit that `at` stands at: page (-1: none) and slot of its first row
-  int page[2], slot[2], rows;
-  auto look_up = [&]() {
-    rows = at.total - at.unit * UNIT;   // may be more than a unit's
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int b = lane + 32 * j, pos = at.unit * UNIT + b * box;
-      page[j] = -1;
-      slot[j] = 0;
-      if (b < boxes && pos < at.total) {
-        page[j] = kv_page(a.pool, at.s, pos);
-        slot[j] = (int)((unsigned)pos % (unsigned)page_size);
-      }
+  // what a lane knows of its unit: page (-1: none) and slot of its box's first row, cache head, rows up to the sequence's end (0: the
+  // run is over)
+  struct Found {
+    int page[2], slot[2], head, rows;
+  };
+  // `at` goes from the run's start to this lane's unit, then a group at a time
+  auto advance = [&](int count) {
+    while (count > 0 && at.pos < end) {
+      const int step = count < at.units - at.unit ? count : at.units - at.unit;
+      at.skip(line, step);
+      count -= step;
     }
   };
-  look_up();
-  while (at.pos < end) {
-    const int head = at.head, pg0 = page[0], pg1 = page[1], sl0 = slot[0], sl1 = slot[1], here = rows;
-    at.next(line);
-    if (at.pos < end) look_up();   // the next unit's entries are on their way while this one's boxes go out
-    uint64_t in = 0;
-    if (pg0 >= 0) in |= low_bits(box) << (lane * box);
-    if (pg1 >= 0) in |= low_bits(box) << ((lane + 32) * box);
-    in = (uint64_t)__reduce_or_sync(0xffffffffu, (uint32_t)(in >> 32)) << 32 | __reduce_or_sync(0xffffffffu, (uint32_t)in);
-    if (!wait(&ring.empty[at_stage.i], at_stage.phase, 1)) break;
-    const uint32_t bar = ptx::smem_u32(&ring.full[at_stage.i]), dst = stages + at_stage.i * 2 * TILE;
-    if (lane == 0) {
-      ring.there[sent % ring.NOTES] = in & low_bits(here);
-      ptx::mbar_arrive_expect_tx(bar, 2 * TILE + a.expect_extra);
-    }
-    __syncwarp();
-    // a copy a lane: keys before values, then box, then which 64 elements
-    for (int i = lane; i - lane < boxes * PARTS; i += 32) {
-      const int v = i >= boxes * (PARTS / 2), k = i - v * boxes * (PARTS / 2), b = k / (PARTS / 2), x = k % (PARTS / 2);
-      const int p0 = __shfl_sync(0xffffffffu, pg0, b & 31), p1 = __shfl_sync(0xffffffffu, pg1, b & 31);
-      const int s0 = __shfl_sync(0xffffffffu, sl0, b & 31), s1 = __shfl_sync(0xffffffffu, sl1, b & 31);
-      if (i < boxes * PARTS) {
-        const int pg = b < 32 ? p0 : p1, sl = b < 32 ? s0 : s1;
-        tma_load_4d(dst + v * TILE + x * (UNIT * 128) + b * box * 128, v ? vm : km, bar, x * 128, sl, head, pg < 0 ? a.pool.pages : pg);
+  auto look_up = [&]() {
+    Found f;
+    f.rows = at.pos < end ? at.total - at.unit * UNIT : 0;
+    f.head = at.head;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int b = box0 + 32 * j, pos = at.unit * UNIT + b * box;
+      f.page[j] = -1;
+      f.slot[j] = 0;
+      if (b < boxes && b * box < f.rows) {
+        f.page[j] = kv_page(a.pool, at.s, pos);
+        f.slot[j] = (int)((unsigned)pos % (unsigned)page_size);
       }
     }
-    ++sent;
-    at_stage.next();
+    return f;
+  };
+  bool more = true;
+  advance(lane / boxes);   // (0 for 32 boxes and more)
+  Found next = look_up();
+  while (more) {
+    const Found now = next;
+    advance(group);
+    next = look_up();   // the next group's entries are on their way while this one's boxes go out
+    for (int g = 0; g < group; ++g) {
+      const int first = boxes < 32 ? g * boxes : 0;   // the lane that knows the unit's first box
+      const int here = __shfl_sync(0xffffffffu, now.rows, first), head = __shfl_sync(0xffffffffu, now.head, first);
+      if (here == 0) {
+        more = false;
+        break;
+      }
+      uint64_t in = 0;
+      if (which == 0) {
+        const bool mine = boxes >= 32 || lane / boxes == g;
+        if (mine && now.page[0] >= 0) in |= low_bits(box) << (box0 * box);
+        if (mine && now.page[1] >= 0) in |= low_bits(box) << ((box0 + 32) * box);
+        in = (uint64_t)__reduce_or_sync(0xffffffffu, (uint32_t)(in >> 32)) << 32 | __reduce_or_sync(0xffffffffu, (uint32_t)in);
+      }
+      if (!wait(&ring.empty[at_stage.i], at_stage.phase, 1)) {
+        more = false;
+        break;
+      }
+      const uint32_t bar = ptx::smem_u32(&ring.full[at_stage.i]), dst = stages + (at_stage.i * 2 + which) * TILE;
+      if (lane == 0) {
+        if (which == 0) ring.there[sent % ring.NOTES] = in & low_bits(here);
+        ptx::mbar_arrive_expect_tx(bar, TILE + a.expect_extra);
+      }
+      __syncwarp();
+#pragma unroll 4
+      for (int b = 0; b < boxes; ++b) {
+        const int pg = __shfl_sync(0xffffffffu, b < 32 ? now.page[0] : now.page[1], (first + b) & 31);
+        const int sl = __shfl_sync(0xffffffffu, b < 32 ? now.slot[0] : now.slot[1], (first + b) & 31);
+#pragma unroll
+        for (int x = 0; x < PARTS; ++x)
+          tma_load_4d(dst + x * (UNIT * 128) + b * box * 128, map, bar, x * 128, sl, head, pg < 0 ? a.pool.pages : pg);
+      }
+      ++sent;
+      at_stage.next();
+    }
   }
   // what is still on its way (when a wait ran out somewhere) lands before the block is gone
   int flag = 0;

@@ -23,7 +23,8 @@ namespace b200q {
 using namespace attn;
 namespace {
 
-constexpr int ROWS = UMMA_ROWS, COMPUTERS = 2 * ROWS, BLOCK = COMPUTERS + 96;   // two streams of rows, a loading warp, one a stream issuing products
+constexpr int ROWS = UMMA_ROWS, COMPUTERS = 2 * ROWS, MAKERS = COMPUTERS / 32 + LOADERS;   // two streams of rows, loading warps,
+constexpr int BLOCK = 32 * (MAKERS + 2);                                                      // a warp a stream that issues products
 constexpr float SLACK = 8.f;                         // log2 of how far weights may exceed 1
 
 // B operand that is contiguous along N: blocks of 64 elements (128-byte swizzle) `lead` bytes apart, groups of 8 rows of K 1024 apart
@@ -178,8 +179,10 @@ tree_attention_umma_kernel(const __grid_constant__ CUtensorMap km, const __grid_
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + (-ptx::smem_u32(smem_raw) & 1023);   // the swizzle goes by the address
   __shared__ Ring<RING> ring;
-  // of a stream: queries in place; a unit's scores made, its weights in place, its products done
-  __shared__ uint64_t q_full[2], s_full[2][2], p_full[2], o_done[2], drained[2];
+  // Of a stream: queries in place; a unit's scores made, its weights in place, its products done.  The last three alternate between two
+  // barriers, step by step: a barrier tells two phases apart, and the roles can be two steps away from each other (a step's scores are
+  // asked for when the products two steps before are done).
+  __shared__ uint64_t q_full[2], s_full[2][2], p_full[2][2], o_done[2][2], drained[2];
   __shared__ long long scan_buf[BLOCK / 32];
   __shared__ float2 other_ml[2][ROWS];               // not PAIR: what the streams tell each other at an item's end
   __shared__ uint32_t bad[2][2], tmem_slot;          // rows of a stream's unit whose values hold infinities or NaN (PAIR: the first)
@@ -196,8 +199,10 @@ tree_attention_umma_kernel(const __grid_constant__ CUtensorMap km, const __grid_
       ptx::mbar_init(ptx::smem_u32(&q_full[j]), PAIR ? ROWS : COMPUTERS);
       ptx::mbar_init(ptx::smem_u32(&s_full[j][0]), 1);
       ptx::mbar_init(ptx::smem_u32(&s_full[j][1]), 1);
-      ptx::mbar_init(ptx::smem_u32(&p_full[j]), ROWS);
-      ptx::mbar_init(ptx::smem_u32(&o_done[j]), 1);
+      ptx::mbar_init(ptx::smem_u32(&p_full[j][0]), ROWS);
+      ptx::mbar_init(ptx::smem_u32(&p_full[j][1]), ROWS);
+      ptx::mbar_init(ptx::smem_u32(&o_done[j][0]), 1);
+      ptx::mbar_init(ptx::smem_u32(&o_done[j][1]), 1);
       ptx::mbar_init(ptx::smem_u32(&drained[j]), 1);
       bad[j][0] = bad[j][1] = 0;
     }
@@ -216,7 +221,7 @@ tree_attention_umma_kernel(const __grid_constant__ CUtensorMap km, const __grid_
   if (u0 >= u1) return;
   // Tensor memory before the successor may come: a successor that takes all of it while this block still waits for its share would
   // wait for this block's end.
-  if (warp == COMPUTERS / 32 + 1) {
+  if (warp == MAKERS) {
     ptx::tmem_alloc(ptx::smem_u32(&tmem_slot), S::COLUMNS);
     ptx::tmem_relinquish();
   }
@@ -229,30 +234,28 @@ tree_attention_umma_kernel(const __grid_constant__ CUtensorMap km, const __grid_
   Place at;
   at.find(line, sums, u0);
   // A wait that runs out ends all waiting: the roles go on without (or stop, where they would load or multiply), and the status says
-  // so.  A warp agrees on it.
+  // so.
   bool dead = false;
-  auto wait = [&](uint64_t* bar, uint32_t parity, int where) {
-    const bool here = !dead && ptx::mbar_wait_bounded_fast<20>(ptx::smem_u32(bar), parity, &abort_flag, where, a.wait_ns);
-    dead = !__all_sync(0xffffffffu, here);
-    return !dead;
-  };
+  auto wait = [&](uint64_t* bar, uint32_t parity, int where) { return warp_wait(bar, parity, dead, &abort_flag, where, a.wait_ns); };
 
   if (warp == COMPUTERS / 32) {
-    load_units<DIM>(a, &km, &vm, line, at, u1, stages, ring, wait);
-  } else if (warp > COMPUTERS / 32) {
+    load_units<DIM>(a, &km, line, at, u1, stages, ring, 0, wait);
+  } else if (warp == COMPUTERS / 32 + 1) {
+    load_units<DIM>(a, &vm, line, at, u1, stages, ring, 1, wait);
+  } else if (warp >= MAKERS) {
     // ---------------------------------------------------------------- products of a stream
     // Scores are asked for one step ahead, within an item.
     constexpr uint32_t FORMAT = F16 ? 0 : 1;
     constexpr uint32_t idesc_s = ptx::make_idesc(1, FORMAT, FORMAT, ROWS, UNIT);
     constexpr uint32_t idesc_o = ptx::make_idesc(1, FORMAT, FORMAT, ROWS, DIM) | IDESC_B_MN;
-    const uint32_t j = warp - COMPUTERS / 32 - 1, columns = tmem + j * S::STREAM;
+    const uint32_t j = warp - MAKERS, columns = tmem + j * S::STREAM;
     const uint64_t q_desc = ptx::make_smem_desc_kmajor(q_tile + (PAIR ? j * S::QUERIES : 0), 1024, 2);
     uint32_t asked = 0, made = 0, items = 0;      // steps whose scores were asked for, whose products were; items with steps so far
     uint32_t unit0 = 0;                           // units of the run before the item
     auto unit_of = [&](uint32_t step) { return PAIR ? step : 2 * step + j; };   // the unit of the run that a step takes
     auto scores = [&]() {
       // The buffer held the weights of the step before the last: its products have to be done.  (Those of the last step, at a new item.)
-      if (made && !wait(&o_done[j], (made - 1) & 1, 6)) return;
+      if (made && !wait(&o_done[j][(made - 1) & 1], (made - 1) >> 1 & 1, 6)) return;
       const uint32_t u = unit_of(asked);
       if (!wait(&ring.full[u % RING], u / RING & 1, 3)) return;
       ptx::tc_fence_after_sync();
@@ -273,13 +276,13 @@ tree_attention_umma_kernel(const __grid_constant__ CUtensorMap km, const __grid_
       while (made < end && !dead) {
         if (asked == made) scores();
         if (asked < end && !dead) scores();
-        if (dead || !wait(&p_full[j], made & 1, 7)) break;
+        if (dead || !wait(&p_full[j][made & 1], made >> 1 & 1, 7)) break;
         ptx::tc_fence_after_sync();
         const uint32_t u = unit_of(made);
         const uint64_t v_desc = make_smem_desc_mnmajor(stages + (u % RING * 2 + 1) * S::TILE, UNIT * 128);
         umma_pv(columns + S::O, columns + (made & 1) * UNIT, (uint32_t)v_desc, (uint32_t)(v_desc >> 32), idesc_o, made > first);
         commit(&ring.empty[u % RING]);
-        commit(&o_done[j]);
+        commit(&o_done[j][made & 1]);
         ++made;
       }
       unit0 += units;
@@ -395,7 +398,7 @@ tree_attention_umma_kernel(const __grid_constant__ CUtensorMap km, const __grid_
           m = now;
           l *= alpha;
           if (!fresh) {
-            wait(&o_done[stream], (done - 1) & 1, 10);
+            wait(&o_done[stream][(done - 1) & 1], (done - 1) >> 1 & 1, 10);
             ptx::tc_fence_after_sync();
 #pragma unroll 1
             for (int c = 0; c < DIM; c += 16) {
@@ -424,12 +427,10 @@ tree_attention_umma_kernel(const __grid_constant__ CUtensorMap km, const __grid_
         ptx::tmem_st_32x32b_x16(s_tmem, p[0]);
         ptx::tmem_st_32x32b_x16(s_tmem + 16, p[1]);
         ptx::tmem_st_wait();
-        // No further ahead of the products than one step (their values may be late): the barriers tell two phases apart, not three.
-        if (done) wait(&o_done[stream], (done - 1) & 1, 13);
         ptx::tc_fence_before_sync();
-        ptx::mbar_arrive(ptx::smem_u32(&p_full[stream]));
+        ptx::mbar_arrive(ptx::smem_u32(&p_full[stream][done & 1]));
         if (fix) {
-          wait(&o_done[stream], done & 1, 11);
+          wait(&o_done[stream][done & 1], done >> 1 & 1, 11);
           ptx::tc_fence_after_sync();
           for (int row = 0; row < UNIT; ++row) {
             if (!(bad_rows[row >> 5] >> (row & 31) & 1)) continue;
@@ -467,7 +468,7 @@ tree_attention_umma_kernel(const __grid_constant__ CUtensorMap km, const __grid_
       }
 
       // ---- the end of the item, or of this block's part
-      if (!fresh) wait(&o_done[stream], (done - 1) & 1, 12);
+      if (!fresh) wait(&o_done[stream][(done - 1) & 1], (done - 1) >> 1 & 1, 12);
       ptx::tc_fence_after_sync();
       const bool whole = started == 0 && units == at.units;
       // not PAIR: both streams know both halves of the row, and each takes half of the columns out
@@ -531,7 +532,7 @@ tree_attention_umma_kernel(const __grid_constant__ CUtensorMap km, const __grid_
   ptx::tc_fence_before_sync();
   __syncthreads();
   ptx::tc_fence_after_sync();
-  if (warp == COMPUTERS / 32 + 1) ptx::tmem_dealloc(tmem, S::COLUMNS);
+  if (warp == MAKERS) ptx::tmem_dealloc(tmem, S::COLUMNS);
 }
 
 template <bool F16, int DIM, bool PAIR>
