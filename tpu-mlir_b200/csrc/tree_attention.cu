@@ -414,45 +414,97 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap km, const __grid_const
   if (dead && lane == 0 && a.io.status) atomicMax(a.io.status, abort_flag);
 }
 
-// Joins the parts of the items that were cut: block x looks after the item that starts in block x's run, a warp takes a row.
+// Joins the parts of the items that were cut: block x looks after the item that starts in block x's run.  A warp takes a row; with more
+// than JOIN_MANY parts (one long context over the whole GPU) four warps share a row's parts and meet in shared memory: 49 rows of 37
+// parts took 15 us a warp a row, %%% so.  Parts are taken four at a time, their loads in flight together, with a running maximum.
+constexpr int JOIN_WARPS = 8, JOIN_SHARE = 4, JOIN_MANY = 8, JOIN_AT_ONCE = 4;
 template <bool F16, int DIM>
-__global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ AttnArgs a, int tile_rows) {
+__global__ void __launch_bounds__(32 * JOIN_WARPS) join_kernel(const __grid_constant__ AttnArgs a, int tile_rows) {
   constexpr int PER = DIM / 32;
+  __shared__ float shared[JOIN_WARPS][DIM + 4];
   ptx::griddep_launch_dependents();
   ptx::griddep_wait();
   const SplitItem it = a.items[blockIdx.x];
-  const int rt = blockIdx.y * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31, r = it.row0 + rt, dim = a.cache.head_dim;
-  if (it.parts == 0 || r >= it.rows) return;
-  // part 0 lies in its block's second place, the others in their blocks' first
-  auto part = [&](int i) { return a.partial + ((int64_t)((blockIdx.x + i) * 2 + (i == 0)) * tile_rows + rt) * (DIM + 4); };
-  float top = -INFINITY;
-  for (int i = lane; i < it.parts; i += 32) top = fmaxf(top, part(i)[DIM]);
+  if (it.parts == 0) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, dim = a.cache.head_dim;
+  const int share = it.parts > JOIN_MANY ? JOIN_SHARE : 1, rows_at_once = JOIN_WARPS / share;
+  const int rows = it.rows - it.row0 < tile_rows ? it.rows - it.row0 : tile_rows;
+  for (int r0 = blockIdx.y * rows_at_once; r0 < rows; r0 += gridDim.y * rows_at_once) {
+    const int rt = r0 + warp / share;
+    float acc[PER], top = -INFINITY, sum = 0.f;
 #pragma unroll
-  for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-  const float base = top == -INFINITY ? 0.f : top;
-  float acc[PER], sum = 0.f;
+    for (int e = 0; e < PER; ++e) acc[e] = 0.f;
+    if (rt < rows) {
+      for (int i0 = warp % share; i0 < it.parts; i0 += share * JOIN_AT_ONCE) {
+        float2 ml[JOIN_AT_ONCE];
+        float x[JOIN_AT_ONCE][PER];
 #pragma unroll
-  for (int e = 0; e < PER; ++e) acc[e] = 0.f;
-#pragma unroll 4
-  for (int i = 0; i < it.parts; ++i) {
-    const float* p = part(i);
-    const float2 ml = *reinterpret_cast<const float2*>(p + DIM);
-    const float w = exp2_approx(ml.x - base);
-    sum += w * ml.y;
+        for (int u = 0; u < JOIN_AT_ONCE; ++u) {
+          const int i = i0 + u * share;
+          // part 0 lies in its block's second place, the others in their blocks' first
+          const float* p = a.partial + ((int64_t)((blockIdx.x + i) * 2 + (i == 0)) * tile_rows + rt) * (DIM + 4);
+          ml[u] = make_float2(-INFINITY, 0.f);
+          if (i < it.parts) ml[u] = *reinterpret_cast<const float2*>(p + DIM);
+#pragma unroll
+          for (int e = 0; e < PER; e += 2) {
+            const float2 v = i < it.parts ? *reinterpret_cast<const float2*>(p + e * 32 + lane * 2) : make_float2(0.f, 0.f);
+            x[u][e] = v.x;
+            x[u][e + 1] = v.y;
+          }
+        }
+        float now = top;
+#pragma unroll
+        for (int u = 0; u < JOIN_AT_ONCE; ++u) now = fmaxf(now, ml[u].x);
+        const float base = now == -INFINITY ? 0.f : now, alpha = exp2_approx(top - base);
+        top = now;
+        sum *= alpha;
+#pragma unroll
+        for (int e = 0; e < PER; ++e) acc[e] *= alpha;
+#pragma unroll
+        for (int u = 0; u < JOIN_AT_ONCE; ++u) {
+          const float w = exp2_approx(ml[u].x - base);
+          sum += w * ml[u].y;
+#pragma unroll
+          for (int e = 0; e < PER; ++e) acc[e] += w * x[u][e];
+        }
+      }
+    }
+    if (share > 1) {
+      __syncthreads();   // (the row before may still be read)
+#pragma unroll
+      for (int e = 0; e < PER; e += 2) *reinterpret_cast<float2*>(&shared[warp][e * 32 + lane * 2]) = make_float2(acc[e], acc[e + 1]);
+      if (lane == 0) *reinterpret_cast<float2*>(&shared[warp][DIM]) = make_float2(top, sum);
+      __syncthreads();
+      if (warp % share) continue;
+      float now = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < JOIN_SHARE; ++w) now = fmaxf(now, shared[warp + w][DIM]);
+      const float base = now == -INFINITY ? 0.f : now;
+      sum = 0.f;
+#pragma unroll
+      for (int e = 0; e < PER; ++e) acc[e] = 0.f;
+#pragma unroll
+      for (int w = 0; w < JOIN_SHARE; ++w) {
+        const float f = exp2_approx(shared[warp + w][DIM] - base);
+        sum += f * shared[warp + w][DIM + 1];
+#pragma unroll
+        for (int e = 0; e < PER; e += 2) {
+          const float2 v = *reinterpret_cast<const float2*>(&shared[warp + w][e * 32 + lane * 2]);
+          acc[e] += f * v.x;
+          acc[e + 1] += f * v.y;
+        }
+      }
+    }
+    if (rt >= rows) continue;
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    const int r = it.row0 + rt;
+    uint16_t* dst = static_cast<uint16_t*>(a.io.out) + (int64_t)(it.first_row + r / a.group) * a.io.out_row_stride +
+                    (it.head * a.group + r % a.group) * a.io.out_head_stride;
 #pragma unroll
     for (int e = 0; e < PER; e += 2) {
-      const float2 x = *reinterpret_cast<const float2*>(p + e * 32 + lane * 2);
-      acc[e] += w * x.x;
-      acc[e + 1] += w * x.y;
+      const int d = e * 32 + lane * 2;
+      if (d < dim) *reinterpret_cast<uint32_t*>(dst + d) = pack_pair<F16>(acc[e] * inv, acc[e + 1] * inv);
     }
-  }
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  uint16_t* dst = static_cast<uint16_t*>(a.io.out) + (int64_t)(it.first_row + r / a.group) * a.io.out_row_stride +
-                  (it.head * a.group + r % a.group) * a.io.out_head_stride;
-#pragma unroll
-  for (int e = 0; e < PER; e += 2) {
-    const int d = e * 32 + lane * 2;
-    if (d < dim) *reinterpret_cast<uint32_t*>(dst + d) = pack_pair<F16>(acc[e] * inv, acc[e + 1] * inv);
   }
 }
 
@@ -499,11 +551,15 @@ int launch_dim(const AttnArgs& a, int sms, cudaStream_t s) {
 
 template <bool F16>
 int launch_join_of(const AttnArgs& a, int blocks, int tile_rows, int dim, cudaStream_t s) {
-  const dim3 grid(blocks, tile_rows / 4);
+  // What the host knows: how many rows a tile has at most, and about how many items there are.  Fewer items than an eighth of the blocks
+  // are cut into more than eight parts each, and two rows are a block's work instead of eight.
+  const int64_t most = a.io.rows * a.group, rows = most < tile_rows ? most : tile_rows, items = a.cache.heads * (a.pool.sequences + most / tile_rows);
+  const int at_once = items * JOIN_MANY < blocks ? JOIN_WARPS / JOIN_SHARE : JOIN_WARPS;
+  const dim3 grid(blocks, (unsigned)((rows + at_once - 1) / at_once)), block(32 * JOIN_WARPS);
   switch (dim) {
-    case 64: return launch_dependent(join_kernel<F16, 64>, grid, dim3(128), 0, s, a, tile_rows);
-    case 128: return launch_dependent(join_kernel<F16, 128>, grid, dim3(128), 0, s, a, tile_rows);
-    default: return launch_dependent(join_kernel<F16, 256>, grid, dim3(128), 0, s, a, tile_rows);
+    case 64: return launch_dependent(join_kernel<F16, 64>, grid, block, 0, s, a, tile_rows);
+    case 128: return launch_dependent(join_kernel<F16, 128>, grid, block, 0, s, a, tile_rows);
+    default: return launch_dependent(join_kernel<F16, 256>, grid, block, 0, s, a, tile_rows);
   }
 }
 
