@@ -140,10 +140,14 @@ __device__ __forceinline__ void tmem_ld_wait_64(uint32_t (&x)[32], uint32_t (&y)
                :
                : "memory");
 }
-// Barriers 1 and 2 are a stream's, 3 is for both.
+// Barriers 1 and 2 are a stream's, 3 is for both, 4 and 5 pass the turn to the first and to the second stream.
 template <int THREADS>
 __device__ __forceinline__ void rows_sync(int id) {
   asm volatile("barrier.cta.sync %0, %1;" ::"r"(id), "n"(THREADS) : "memory");
+}
+template <int THREADS>
+__device__ __forceinline__ void rows_arrive(int id) {
+  asm volatile("barrier.cta.arrive %0, %1;" ::"r"(id), "n"(THREADS) : "memory");
 }
 template <int THREADS>
 __device__ __forceinline__ bool rows_or(int id, bool x) {
@@ -412,6 +416,10 @@ tree_attention_umma_kernel(const __grid_constant__ CUtensorMap km, const __grid_
             ptx::tmem_st_wait();
           }
         }
+        // ---- The streams exponentiate in turn, step by step: left alone they fall into step, share the exponential unit and then both leave
+        // it idle (2060 clocks a step where this takes %%%).
+        const uint32_t turn = PAIR ? 2 * unit + stream : unit;
+        if (turn) rows_sync<COMPUTERS>(4 + (turn & 1));
         // ---- weights (rounded to the 16-bit type: what the tensor cores take; the rounding is unbiased and averages out over positions)
         const float base = m == -INFINITY ? 0.f : m;
         uint32_t p[2][16];   // two weights a word
@@ -423,6 +431,7 @@ tree_attention_umma_kernel(const __grid_constant__ CUtensorMap km, const __grid_
           sum1 += y;
           p[j / 32][j / 2 % 16] = pack_pair<F16>(x, y);
         }
+        rows_arrive<COMPUTERS>(4 + (turn + 1 & 1));
         l += sum0 + sum1;
         ptx::tmem_st_32x32b_x16(s_tmem, p[0]);
         ptx::tmem_st_32x32b_x16(s_tmem + 16, p[1]);
