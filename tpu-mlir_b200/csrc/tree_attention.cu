@@ -152,6 +152,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap km, const __grid_const
         const bool real = r < at.nodes * group;
         const int t = r / group, row = at.first_row + (real ? t : 0);
         node[h] = t;
+        if (a.io.mask && a.io.mask_stride && (lane & 3) == 0) prefetch(a.io.mask + (int64_t)row * a.io.mask_stride);
         m[h] = -INFINITY;
         l[h] = 0.f;
         const uint16_t* src = static_cast<const uint16_t*>(a.io.q) + (int64_t)row * a.io.q_row_stride + (at.head * group + r % group) * a.io.q_head_stride;
@@ -399,10 +400,11 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap km, const __grid_const
               if (d < dim) *reinterpret_cast<uint32_t*>(dst + d) = pack_pair<F16>(o[k][2 * h] * inv, o[k][2 * h + 1] * inv);
             }
           } else {
-            float* dst = a.partial + ((int64_t)(blockIdx.x * 2 + (started == 0)) * S::ROWS + rt) * (DIM + 4);
+            float* dst = a.partial + (blockIdx.x * 2 + (started == 0)) * part_size(S::ROWS, DIM);
 #pragma unroll
-            for (int k = 0; k < DIM / 8; ++k) *reinterpret_cast<float2*>(dst + k * 8 + (lane & 3) * 2) = make_float2(o[k][2 * h], o[k][2 * h + 1]);
-            if ((lane & 3) == 0) *reinterpret_cast<float2*>(dst + DIM) = make_float2(m[h], l[h]);
+            for (int k = 0; k < DIM / 8; ++k)
+              *reinterpret_cast<float2*>(dst + part_at(S::ROWS, rt, k * 2 + (lane & 3) / 2) + (lane & 1) * 2) = make_float2(o[k][2 * h], o[k][2 * h + 1]);
+            if ((lane & 3) == 0) *reinterpret_cast<float2*>(dst + part_at(S::ROWS, rt, DIM / 4)) = make_float2(m[h], l[h]);
           }
         }
       }
@@ -414,97 +416,80 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap km, const __grid_const
   if (dead && lane == 0 && a.io.status) atomicMax(a.io.status, abort_flag);
 }
 
-// Joins the parts of the items that were cut: block x looks after the item that starts in block x's run.  A warp takes a row; with more
-// than JOIN_MANY parts (one long context over the whole GPU) four warps share a row's parts and meet in shared memory: 49 rows of 37
-// parts took 15 us a warp a row, %%% so.  Parts are taken four at a time, their loads in flight together, with a running maximum.
-constexpr int JOIN_WARPS = 8, JOIN_SHARE = 4, JOIN_MANY = 8, JOIN_AT_ONCE = 4;
-template <bool F16, int DIM>
-__global__ void __launch_bounds__(32 * JOIN_WARPS) join_kernel(const __grid_constant__ AttnArgs a, int tile_rows) {
-  constexpr int PER = DIM / 32;
-  __shared__ float shared[JOIN_WARPS][DIM + 4];
+// Joins the parts of the items that were cut: block x looks after the item that starts in block x's run.  A warp takes eight rows, four
+// lanes of each: four columns a lane; or, with more than JOIN_MANY parts (one long context over the whole GPU), one four-column piece
+// whose parts the lanes share.  Parts are taken four at a time, their loads in flight together, with a running maximum.
+constexpr int JOIN_THREADS = 256, JOIN_MANY = 8, JOIN_AT_ONCE = 4;
+template <bool F16>
+__global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const __grid_constant__ AttnArgs a, int tile_rows, int dim_padded) {
   ptx::griddep_launch_dependents();
   ptx::griddep_wait();
   const SplitItem it = a.items[blockIdx.x];
   if (it.parts == 0) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, dim = a.cache.head_dim;
-  const int share = it.parts > JOIN_MANY ? JOIN_SHARE : 1, rows_at_once = JOIN_WARPS / share;
+  const bool many = it.parts > JOIN_MANY;
   const int rows = it.rows - it.row0 < tile_rows ? it.rows - it.row0 : tile_rows;
-  for (int r0 = blockIdx.y * rows_at_once; r0 < rows; r0 += gridDim.y * rows_at_once) {
-    const int rt = r0 + warp / share;
-    float acc[PER], top = -INFINITY, sum = 0.f;
+  const int wide = (dim + 3) / 4, pieces = many ? wide : (wide + 3) / 4, works = (rows + 7) / 8 * pieces;   // of a warp
+  const int share = many ? 4 : 1, mine = many ? lane >> 3 : 0;
+  for (int w = blockIdx.y * (JOIN_THREADS / 32) + warp; w < works; w += gridDim.y * (JOIN_THREADS / 32)) {
+    const int rt = w / pieces * 8 + (lane & 7), four = many ? w % pieces : w % pieces * 4 + (lane >> 3);
+    const bool there = rt < rows && four < wide;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    float top = -INFINITY, sum = 0.f;
+    for (int i0 = mine; i0 < it.parts; i0 += share * JOIN_AT_ONCE) {
+      float2 ml[JOIN_AT_ONCE];
+      float4 x[JOIN_AT_ONCE];
 #pragma unroll
-    for (int e = 0; e < PER; ++e) acc[e] = 0.f;
-    if (rt < rows) {
-      for (int i0 = warp % share; i0 < it.parts; i0 += share * JOIN_AT_ONCE) {
-        float2 ml[JOIN_AT_ONCE];
-        float x[JOIN_AT_ONCE][PER];
-#pragma unroll
-        for (int u = 0; u < JOIN_AT_ONCE; ++u) {
-          const int i = i0 + u * share;
-          // part 0 lies in its block's second place, the others in their blocks' first
-          const float* p = a.partial + ((int64_t)((blockIdx.x + i) * 2 + (i == 0)) * tile_rows + rt) * (DIM + 4);
-          ml[u] = make_float2(-INFINITY, 0.f);
-          if (i < it.parts) ml[u] = *reinterpret_cast<const float2*>(p + DIM);
-#pragma unroll
-          for (int e = 0; e < PER; e += 2) {
-            const float2 v = i < it.parts ? *reinterpret_cast<const float2*>(p + e * 32 + lane * 2) : make_float2(0.f, 0.f);
-            x[u][e] = v.x;
-            x[u][e + 1] = v.y;
-          }
-        }
-        float now = top;
-#pragma unroll
-        for (int u = 0; u < JOIN_AT_ONCE; ++u) now = fmaxf(now, ml[u].x);
-        const float base = now == -INFINITY ? 0.f : now, alpha = exp2_approx(top - base);
-        top = now;
-        sum *= alpha;
-#pragma unroll
-        for (int e = 0; e < PER; ++e) acc[e] *= alpha;
-#pragma unroll
-        for (int u = 0; u < JOIN_AT_ONCE; ++u) {
-          const float w = exp2_approx(ml[u].x - base);
-          sum += w * ml[u].y;
-#pragma unroll
-          for (int e = 0; e < PER; ++e) acc[e] += w * x[u][e];
+      for (int u = 0; u < JOIN_AT_ONCE; ++u) {
+        const int i = i0 + u * share;
+        // part 0 lies in its block's second place, the others in their blocks' first
+        const float* p = a.partial + ((blockIdx.x + i) * 2 + (i == 0)) * part_size(tile_rows, dim_padded);
+        ml[u] = make_float2(-INFINITY, 0.f);
+        x[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (there && i < it.parts) {
+          ml[u] = *reinterpret_cast<const float2*>(p + part_at(tile_rows, rt, dim_padded / 4));
+          x[u] = *reinterpret_cast<const float4*>(p + part_at(tile_rows, rt, four));
         }
       }
-    }
-    if (share > 1) {
-      __syncthreads();   // (the row before may still be read)
+      float now = top;
 #pragma unroll
-      for (int e = 0; e < PER; e += 2) *reinterpret_cast<float2*>(&shared[warp][e * 32 + lane * 2]) = make_float2(acc[e], acc[e + 1]);
-      if (lane == 0) *reinterpret_cast<float2*>(&shared[warp][DIM]) = make_float2(top, sum);
-      __syncthreads();
-      if (warp % share) continue;
-      float now = -INFINITY;
+      for (int u = 0; u < JOIN_AT_ONCE; ++u) now = fmaxf(now, ml[u].x);
+      const float base = now == -INFINITY ? 0.f : now, alpha = exp2_approx(top - base);
+      top = now;
+      sum *= alpha;
+      acc = make_float4(acc.x * alpha, acc.y * alpha, acc.z * alpha, acc.w * alpha);
 #pragma unroll
-      for (int w = 0; w < JOIN_SHARE; ++w) now = fmaxf(now, shared[warp + w][DIM]);
-      const float base = now == -INFINITY ? 0.f : now;
-      sum = 0.f;
-#pragma unroll
-      for (int e = 0; e < PER; ++e) acc[e] = 0.f;
-#pragma unroll
-      for (int w = 0; w < JOIN_SHARE; ++w) {
-        const float f = exp2_approx(shared[warp + w][DIM] - base);
-        sum += f * shared[warp + w][DIM + 1];
-#pragma unroll
-        for (int e = 0; e < PER; e += 2) {
-          const float2 v = *reinterpret_cast<const float2*>(&shared[warp + w][e * 32 + lane * 2]);
-          acc[e] += f * v.x;
-          acc[e + 1] += f * v.y;
-        }
+      for (int u = 0; u < JOIN_AT_ONCE; ++u) {
+        const float f = exp2_approx(ml[u].x - base);
+        sum += f * ml[u].y;
+        acc.x += f * x[u].x;
+        acc.y += f * x[u].y;
+        acc.z += f * x[u].z;
+        acc.w += f * x[u].w;
       }
     }
-    if (rt >= rows) continue;
+    if (many) {
+      // the lanes that shared a row's parts: a common maximum, then the sums in a fixed order
+      float now = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+      now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, 16));
+      const float f = exp2_approx(top - (now == -INFINITY ? 0.f : now));
+      sum *= f;
+      acc = make_float4(acc.x * f, acc.y * f, acc.z * f, acc.w * f);
+#pragma unroll
+      for (int d = 8; d <= 16; d += 8) {
+        sum += __shfl_xor_sync(0xffffffffu, sum, d);
+        acc.x += __shfl_xor_sync(0xffffffffu, acc.x, d);
+        acc.y += __shfl_xor_sync(0xffffffffu, acc.y, d);
+        acc.z += __shfl_xor_sync(0xffffffffu, acc.z, d);
+        acc.w += __shfl_xor_sync(0xffffffffu, acc.w, d);
+      }
+    }
+    if (!there || mine) continue;
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
     const int r = it.row0 + rt;
     uint16_t* dst = static_cast<uint16_t*>(a.io.out) + (int64_t)(it.first_row + r / a.group) * a.io.out_row_stride +
-                    (it.head * a.group + r % a.group) * a.io.out_head_stride;
-#pragma unroll
-    for (int e = 0; e < PER; e += 2) {
-      const int d = e * 32 + lane * 2;
-      if (d < dim) *reinterpret_cast<uint32_t*>(dst + d) = pack_pair<F16>(acc[e] * inv, acc[e + 1] * inv);
-    }
+                    (it.head * a.group + r % a.group) * a.io.out_head_stride + four * 4;
+    *reinterpret_cast<uint2*>(dst) = make_uint2(pack_pair<F16>(acc.x * inv, acc.y * inv), pack_pair<F16>(acc.z * inv, acc.w * inv));
   }
 }
 
@@ -512,8 +497,9 @@ constexpr int BLOCKS_PER_SM = 2;
 
 // Layout of the workspace for `blocks` blocks: what was cut, then the partial sums.
 int64_t workspace_bytes(int blocks, int dim) {
-  const int64_t items = ((int64_t)blocks * sizeof(SplitItem) + 255) / 256 * 256, rows = dim > 128 ? 32 : UMMA_ROWS;
-  return items + (int64_t)blocks * 2 * rows * (dim + 4) * 4;
+  const int64_t items = ((int64_t)blocks * sizeof(SplitItem) + 255) / 256 * 256;
+  const int rows = dim > 128 ? 32 : UMMA_ROWS;   // (two tiles a block of half as many blocks are the same)
+  return items + blocks * 2 * part_size(rows, dim) * 4;
 }
 int padded_dim(int head_dim) { return head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256; }
 
@@ -549,20 +535,6 @@ int launch_dim(const AttnArgs& a, int sms, cudaStream_t s) {
   }
 }
 
-template <bool F16>
-int launch_join_of(const AttnArgs& a, int blocks, int tile_rows, int dim, cudaStream_t s) {
-  // What the host knows: how many rows a tile has at most, and about how many items there are.  Fewer items than an eighth of the blocks
-  // are cut into more than eight parts each, and two rows are a block's work instead of eight.
-  const int64_t most = a.io.rows * a.group, rows = most < tile_rows ? most : tile_rows, items = a.cache.heads * (a.pool.sequences + most / tile_rows);
-  const int at_once = items * JOIN_MANY < blocks ? JOIN_WARPS / JOIN_SHARE : JOIN_WARPS;
-  const dim3 grid(blocks, (unsigned)((rows + at_once - 1) / at_once)), block(32 * JOIN_WARPS);
-  switch (dim) {
-    case 64: return launch_dependent(join_kernel<F16, 64>, grid, block, 0, s, a, tile_rows);
-    case 128: return launch_dependent(join_kernel<F16, 128>, grid, block, 0, s, a, tile_rows);
-    default: return launch_dependent(join_kernel<F16, 256>, grid, block, 0, s, a, tile_rows);
-  }
-}
-
 }  // namespace
 
 namespace attn {
@@ -575,7 +547,14 @@ int make_map(CUtensorMap* map, const AttnArgs& a, const void* base) {
 }
 
 int launch_join(const AttnArgs& a, int blocks, int tile_rows, int dim, cudaStream_t s) {
-  return a.cache.dtype == B200Q_DT_F16 ? launch_join_of<true>(a, blocks, tile_rows, dim, s) : launch_join_of<false>(a, blocks, tile_rows, dim, s);
+  // What the host knows: how many rows a tile has at most, and about how many items there are.  Few items are cut into many parts each,
+  // and get a block for every eight warps' work; many get half of that each, and keep the launch small.
+  const int64_t most = a.io.rows * a.group, rows = most < tile_rows ? most : tile_rows, items = a.cache.heads * (a.pool.sequences + most / tile_rows);
+  const bool few = items * JOIN_MANY < blocks;
+  const int64_t warps = (rows + 7) / 8 * (dim / (few ? 4 : 16)), per_block = JOIN_THREADS / 32 * (few ? 1 : 2);
+  const dim3 grid(blocks, (unsigned)((warps + per_block - 1) / per_block)), block(JOIN_THREADS);
+  return a.cache.dtype == B200Q_DT_F16 ? launch_dependent(join_kernel<true>, grid, block, 0, s, a, tile_rows, dim)
+                                       : launch_dependent(join_kernel<false>, grid, block, 0, s, a, tile_rows, dim);
 }
 }  // namespace attn
 }  // namespace b200q

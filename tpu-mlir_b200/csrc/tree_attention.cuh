@@ -21,9 +21,15 @@ struct AttnArgs {
   int min_run;        // the shortest run of the line that a block takes, if there is so much
   unsigned long long wait_ns;   // no wait inside the kernel lasts longer
   int expect_extra;             // test aid: bytes that a stage waits for and that never come (0 in normal use)
-  float* partial;     // [blocks][2][rows of a tile][dim + 4]: sums, maximum (log2 domain), total, nothing
+  // partial sums: [block][2][dim / 4 + 1][rows of a tile][4]; the last four of a row are its maximum (log2 domain) and its total.
+  // (Four columns of all rows next to each other: the writers' threads are rows.)
+  float* partial;
   struct SplitItem* items;   // [blocks]
 };
+
+// floats of a part, and where four columns of a row stand in it
+constexpr __host__ __device__ int64_t part_size(int tile_rows, int dim) { return (int64_t)tile_rows * (dim + 4); }
+__device__ __forceinline__ int part_at(int tile_rows, int row, int four) { return (four * tile_rows + row) * 4; }
 
 // The item that starts in a block's run and ends in a later one's.
 struct SplitItem {
@@ -84,6 +90,7 @@ template <bool F16>
 __device__ __forceinline__ float from_bits(uint32_t bits) {
   return F16 ? __half2float(__ushort_as_half((unsigned short)bits)) : __uint_as_float(bits << 16);
 }
+__device__ __forceinline__ void prefetch(const void* p) { asm volatile("prefetch.global.L1 [%0];" ::"l"(p)); }
 __device__ __forceinline__ uint64_t low_bits(int n) { return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1; }
 
 // Which of the 64 positions from `p0` on node `node` sees: all committed ones, and the nodes that its mask names (a chain: up to
@@ -250,8 +257,8 @@ __device__ __forceinline__ void load_units(const AttnArgs& a, const CUtensorMap*
   const int group = boxes < 32 ? 32 / boxes : 1, box0 = lane % boxes;   // units of a group; this lane's box of its unit
   Slot<STAGES> at_stage(1);     // the first pass over the ring finds it empty
   uint32_t sent = 0;
-  // what a lane knows of its unit: page (-1: none) and slot of its box's first row, cache head, rows up to the sequence's end (0: the
-  // run is over)
+  // what a lane knows of its unit: the table's entry for its box (as it stands there, so that nothing waits for it; -1: none) and slot of
+  // the box's first row, cache head, rows up to the sequence's end (0: the run is over)
   struct Found {
     int page[2], slot[2], head, rows;
   };
@@ -273,7 +280,8 @@ __device__ __forceinline__ void load_units(const AttnArgs& a, const CUtensorMap*
       f.page[j] = -1;
       f.slot[j] = 0;
       if (b < boxes && b * box < f.rows) {
-        f.page[j] = kv_page(a.pool, at.s, pos);
+        // (total is within the table)
+        f.page[j] = a.pool.table[at.s * a.pool.table_stride + (unsigned)pos / (unsigned)page_size];
         f.slot[j] = (int)((unsigned)pos % (unsigned)page_size);
       }
     }
@@ -296,8 +304,8 @@ __device__ __forceinline__ void load_units(const AttnArgs& a, const CUtensorMap*
       uint64_t in = 0;
       if (which == 0) {
         const bool mine = boxes >= 32 || lane / boxes == g;
-        if (mine && now.page[0] >= 0) in |= low_bits(box) << (box0 * box);
-        if (mine && now.page[1] >= 0) in |= low_bits(box) << ((box0 + 32) * box);
+        if (mine && (unsigned)now.page[0] < (unsigned)a.pool.pages) in |= low_bits(box) << (box0 * box);
+        if (mine && (unsigned)now.page[1] < (unsigned)a.pool.pages) in |= low_bits(box) << ((box0 + 32) * box);
         in = (uint64_t)__reduce_or_sync(0xffffffffu, (uint32_t)(in >> 32)) << 32 | __reduce_or_sync(0xffffffffu, (uint32_t)in);
       }
       if (!wait(&ring.empty[at_stage.i], at_stage.phase, 1)) {
@@ -316,7 +324,7 @@ __device__ __forceinline__ void load_units(const AttnArgs& a, const CUtensorMap*
         const int sl = __shfl_sync(0xffffffffu, b < 32 ? now.slot[0] : now.slot[1], (first + b) & 31);
 #pragma unroll
         for (int x = 0; x < PARTS; ++x)
-          tma_load_4d(dst + x * (UNIT * 128) + b * box * 128, map, bar, x * 128, sl, head, pg < 0 ? a.pool.pages : pg);
+          tma_load_4d(dst + x * (UNIT * 128) + b * box * 128, map, bar, x * 128, sl, head, (unsigned)pg < (unsigned)a.pool.pages ? pg : a.pool.pages);
       }
       ++sent;
       at_stage.next();

@@ -314,14 +314,28 @@ tree_attention_umma_kernel(const __grid_constant__ CUtensorMap km, const __grid_
       const int started = at.unit, units = (int)(left < at.units - at.unit ? left : at.units - at.unit);
       const long long first = at.pos - at.unit;   // where the item's units start in the line
       const int r0 = at.tile * TILE_ROWS + (PAIR ? stream * ROWS : 0), rows = at.nodes * group;
-      for (int c = PAIR ? row_in : tid; c < ROWS * PIECES; c += PAIR ? ROWS : COMPUTERS) {
-        const int row = c / PIECES, piece = c % PIECES, r = r0 + row;
-        uint4 x = make_uint4(0, 0, 0, 0);
-        if (r < rows && piece * 8 < dim)
-          x = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.io.q) + (int64_t)(at.first_row + r / group) * a.io.q_row_stride +
-                                              (at.head * group + r % group) * a.io.q_head_stride + piece * 8);
-        *reinterpret_cast<uint4*>(smem + (PAIR ? stream * S::QUERIES : 0) + (piece >> 3) * (ROWS * 128) + row * 128 +
-                                  (((piece & 7) ^ (row & 7)) * 16)) = x;
+      {
+        // 16 bytes a thread and access, eight accesses in flight (one after the other they took 6000 clocks and more)
+        constexpr int LOADING = PAIR ? ROWS : COMPUTERS, STEP = LOADING / PIECES, PASSES = ROWS / STEP, AT_ONCE = PASSES < 8 ? PASSES : 8;
+        const int at0 = PAIR ? row_in : tid, piece = at0 % PIECES, row0 = at0 / PIECES;
+        uint8_t* dst = smem + (PAIR ? stream * S::QUERIES : 0) + (piece >> 3) * (ROWS * 128);
+#pragma unroll
+        for (int p0 = 0; p0 < PASSES; p0 += AT_ONCE) {
+          uint4 x[AT_ONCE];
+#pragma unroll
+          for (int i = 0; i < AT_ONCE; ++i) {
+            const int r = r0 + row0 + (p0 + i) * STEP, t = r / group;
+            x[i] = make_uint4(0, 0, 0, 0);
+            if (r < rows && piece * 8 < dim)
+              x[i] = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.io.q) + (int64_t)(at.first_row + t) * a.io.q_row_stride +
+                                                     (at.head * group + r - t * group) * a.io.q_head_stride + piece * 8);
+          }
+#pragma unroll
+          for (int i = 0; i < AT_ONCE; ++i) {
+            const int row = row0 + (p0 + i) * STEP;
+            *reinterpret_cast<uint4*>(dst + row * 128 + (((piece & 7) ^ (row & 7)) * 16)) = x[i];
+          }
+        }
       }
       ptx::fence_proxy_async_smem();
       // (not PAIR: an item of one unit is one stream's alone)
@@ -333,6 +347,7 @@ tree_attention_umma_kernel(const __grid_constant__ CUtensorMap km, const __grid_
       }
       const int r = r0 + row_in, node = r / group;
       const bool real = r < rows;
+      if (a.io.mask && a.io.mask_stride && real) prefetch(a.io.mask + (int64_t)(at.first_row + node) * a.io.mask_stride);
       float m = -INFINITY, l = 0.f;
       bool fresh = true;
 
@@ -498,7 +513,8 @@ tree_attention_umma_kernel(const __grid_constant__ CUtensorMap km, const __grid_
       const float inv = l == 0.f ? 0.f : 1.f / l;
       uint16_t* dst = static_cast<uint16_t*>(a.io.out) + (int64_t)(at.first_row + (real ? node : 0)) * a.io.out_row_stride +
                       (at.head * group + r % group) * a.io.out_head_stride;
-      float* part = a.partial + ((int64_t)(blockIdx.x * 2 + (started == 0)) * TILE_ROWS + (PAIR ? stream * ROWS : 0) + row_in) * (DIM + 4);
+      float* part = a.partial + (blockIdx.x * 2 + (started == 0)) * part_size(TILE_ROWS, DIM);
+      const int part_row = (PAIR ? stream * ROWS : 0) + row_in;
       const uint32_t theirs = mine ^ S::STREAM;   // (the allocation starts at a multiple of its size)
 #pragma unroll
       for (int c0 = 0; c0 < (PAIR ? DIM : DIM / 2); c0 += 32) {
@@ -525,10 +541,10 @@ tree_attention_umma_kernel(const __grid_constant__ CUtensorMap km, const __grid_
                                                                   pack_pair<F16>(o[e + 4] * inv, o[e + 5] * inv), pack_pair<F16>(o[e + 6] * inv, o[e + 7] * inv));
         } else {
 #pragma unroll
-          for (int e = 0; e < 32; e += 4) *reinterpret_cast<float4*>(part + c + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+          for (int e = 0; e < 32; e += 4) *reinterpret_cast<float4*>(part + part_at(TILE_ROWS, part_row, (c + e) / 4)) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
         }
       }
-      if (real && !whole && (PAIR || stream == 0)) *reinterpret_cast<float2*>(part + DIM) = make_float2(m, l);
+      if (real && !whole && (PAIR || stream == 0)) *reinterpret_cast<float2*>(part + part_at(TILE_ROWS, part_row, DIM / 4)) = make_float2(m, l);
       ptx::tc_fence_before_sync();
       if (!PAIR) rows_sync<COMPUTERS>(3);   // the sums are out of tensor memory, and what was told is read, before either goes on
       if (tid == 0 && started == 0 && !whole)
