@@ -10,11 +10,12 @@
 // device: each block adds up the batch's units for itself.  An item that a run's end cuts leaves fp32 partial sums in the workspace
 // (at most two a block), which a second kernel joins, in the order of the positions.
 //
-// One warp of a block only loads, with TMA boxes of as many rows as both a page and a unit are made of: a lane looks a box's page
-// up and issues its copy, ahead of the products and across items, into a ring of stages of 64 keys and values; four warps
-// compute.  Shared memory holds 64 elements a row, swizzled by 16-byte pieces (piece ^ row % 8), so that ldmatrix meets no bank
-// twice.  (Loading with 16-byte cp.async instead, one or two warps a block, took 640 instructions a warp and unit and held the
-// computing warps up: 108 us where this takes %%%.)
+// Two warps of a block only load, one keys and one values, with TMA boxes of as many rows as both a page and a unit are made of, ahead of
+// the products and across items, into a ring of stages of 64 keys and values; four warps compute.  Shared memory holds 64 elements
+// a row, swizzled by 16-byte pieces (piece ^ row % 8), so that ldmatrix meets no bank twice.  (Loading with 16-byte cp.async took 640
+// instructions a warp and unit: 108 us for 48 sequences of one token, 450 MB, that take 81.5 this way: 5.5 TB/s, 0.84 of the measured rate.)
+//
+// What bounds it: DRAM; 10 us of a launch, the batch's lengths, the first unit's way through table and memory, and the join are fixed.
 #include <math.h>
 
 #include "igemm.h"
@@ -47,6 +48,9 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+// What an item costs, in units (48 sequences of one token: 91 / 84.5 / 81.6 / 81.6 us at 1 / 2 / 3 / 4), and the shortest run of units that is
+// worth a block (one token at 430 positions: 13 us at one unit, 14 at two, 16 at four, 20 at eight).
+constexpr int ITEM_COST = 3, MIN_UNITS = 1;
 constexpr int COMPUTERS = 128, BLOCK = COMPUTERS + 32 * LOADERS;
 
 __device__ __forceinline__ void computers_sync() { asm volatile("barrier.cta.sync 1, 128;" ::: "memory"); }
@@ -105,11 +109,11 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap km, const __grid_const
     ptx::prefetch_tensormap(&vm);
   }
   ptx::griddep_wait();
-  const long long total = lay_out<BLOCK>(a, S::ROWS, seqs, sums, scan_buf);
-  const Line line{seqs, a.pool.sequences, a.cache.heads, group, S::ROWS};
+  const long long total = lay_out<BLOCK>(a, S::ROWS, ITEM_COST, seqs, sums, scan_buf);
+  const Line line{seqs, a.pool.sequences, a.cache.heads, group, S::ROWS, ITEM_COST};
 
   long long run = (total + gridDim.x - 1) / gridDim.x;
-  if (run < a.min_run) run = a.min_run;
+  if (run < MIN_UNITS + ITEM_COST) run = MIN_UNITS + ITEM_COST;
   const long long u0 = (long long)blockIdx.x * run, u1 = u0 + run < total ? u0 + run : total;
   if (tid == 0) a.items[blockIdx.x].parts = 0;
   if (u0 >= u1) return;
@@ -609,7 +613,6 @@ int b200q_tree_attention_dev(const b200q_kv_cache* cache, const b200q_kv_pool* p
   a.box = UNIT;
   while (pool->page_size % a.box) a.box /= 2;   // the greatest power of two that divides a page, up to a unit
   igemm_wait_test(&a.expect_extra, &a.wait_ns);
-  a.min_run = 1 + ITEM_COST;
   a.items = static_cast<SplitItem*>(io.workspace);
   a.partial = reinterpret_cast<float*>(static_cast<uint8_t*>(io.workspace) + ((int64_t)blocks * sizeof(SplitItem) + 255) / 256 * 256);
   cudaStream_t s = static_cast<cudaStream_t>(stream);

@@ -18,7 +18,6 @@ struct AttnArgs {
   int group;          // query heads of a cache head
   float scale_log2;   // scale * log2(e)
   int box;            // rows of a TMA box
-  int min_run;        // the shortest run of the line that a block takes, if there is so much
   unsigned long long wait_ns;   // no wait inside the kernel lasts longer
   int expect_extra;             // test aid: bytes that a stage waits for and that never come (0 in normal use)
   // partial sums: [block][2][dim / 4 + 1][rows of a tile][4]; the last four of a row are its maximum (log2 domain) and its total.
@@ -54,6 +53,11 @@ __device__ __forceinline__ Sequence load_sequence(const AttnArgs& a, int s) {
   return q;
 }
 
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool there) {
+  const int n = there ? 16 : 0;   // 0: the 16 bytes become zeros, nothing is read
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 // A box of a page's rows: x byte of the head, y slot, z head, w page; what lies outside becomes zeros.  Called by a whole warp with
 // the same arguments, issued by one elected thread (a copy from a branch, or one a lane, took 100 clocks each).
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z, int w) {
@@ -113,11 +117,10 @@ __device__ __forceinline__ uint64_t sees(const AttnArgs& a, int row, int node, i
 // ---- the line of units: which unit stands at a position of it
 struct Line {
   const Sequence* seqs;
-  int sequences, heads, group, tile_rows;
+  int sequences, heads, group, tile_rows, cost;
 };
-// An item (sequence, cache head, row tile) takes ITEM_COST positions of the line and one for each unit: what a block spends on an
-// item besides its units (queries, the sums' way out) counts when runs are made equal.
-constexpr int ITEM_COST = 2;
+// An item (sequence, cache head, row tile) takes line.cost positions and one for each unit: what a block spends on an item besides
+// its units (queries, the first scores, the sums' way out) counts when runs are made equal.
 struct Place {
   long long pos;                     // in the line
   int s, head, tile, unit;           // row tile of the sequence, unit of the item
@@ -141,9 +144,12 @@ struct Place {
       else lo = mid + 1;
     }
     enter(line, lo);
-    const long long local = at - (lo ? sums[lo - 1] : 0), item = local / (units + ITEM_COST);
-    const int in = (int)(local - item * (units + ITEM_COST)) - ITEM_COST;
-    head = (int)(item / tiles);
+    const long long local = at - (lo ? sums[lo - 1] : 0);
+    const int stretch = units + line.cost;   // of an item
+    // (a 64-bit division takes hundreds of clocks)
+    const long long item = local <= 0x7fffffff ? (unsigned)local / (unsigned)stretch : local / stretch;
+    const int in = (int)(local - item * stretch) - line.cost;
+    head = (int)(item <= 0x7fffffff ? (unsigned)item / (unsigned)tiles : item / tiles);
     tile = (int)(item - (long long)head * tiles);
     unit = in > 0 ? in : 0;
     pos = at + (in < 0 ? -in : 0);
@@ -154,7 +160,7 @@ struct Place {
     pos += count;
     if ((unit += count) < units) return;
     unit = 0;
-    pos += ITEM_COST;
+    pos += line.cost;
     if (++tile < tiles) return;
     tile = 0;
     if (++head < line.heads) return;
@@ -167,7 +173,7 @@ struct Place {
 
 // Fills seqs and sums (the line's length up to and with each sequence) for all threads of the block; returns the line's length.
 template <int THREADS>
-__device__ __forceinline__ long long lay_out(const AttnArgs& a, int tile_rows, Sequence* seqs, long long* sums, long long* buf) {
+__device__ __forceinline__ long long lay_out(const AttnArgs& a, int tile_rows, int cost, Sequence* seqs, long long* sums, long long* buf) {
   const int n = a.pool.sequences, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int each = (n + THREADS - 1) / THREADS;
   long long mine = 0;
@@ -176,7 +182,7 @@ __device__ __forceinline__ long long lay_out(const AttnArgs& a, int tile_rows, S
     if (s >= n) break;
     const Sequence q = load_sequence(a, s);
     const long long tiles = ((long long)q.nodes * a.group + tile_rows - 1) / tile_rows;
-    mine += a.cache.heads * tiles * ((q.total + UNIT - 1) / UNIT + ITEM_COST);
+    mine += a.cache.heads * tiles * ((q.total + UNIT - 1) / UNIT + cost);
     seqs[s] = q;
     sums[s] = mine;
   }

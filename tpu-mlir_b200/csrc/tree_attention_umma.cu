@@ -6,7 +6,7 @@
 //                 into tensor memory over the scores that they came from, rounded to the 16-bit type
 //   O += P V      128 x dim, P from tensor memory, V as it lies (positions x head: the operand is MN-major)
 // A block (one an SM: the rings of keys and values have to be deep, four to eight units, or their latency sets the pace: with two
-// stages and two blocks an SM this took 204 us where it takes %%%) keeps two streams of this going, each with four warps, two buffers of
+// stages and two blocks an SM 8 trees of 64 nodes over 16000 positions took 204 us where this takes 115) keeps two streams of this going, each with four warps, two buffers of
 // scores and sums of its own.  With more than 128 rows a cache head the streams are two row tiles that share every unit of keys
 // and values (PAIR); with fewer they take the units of one row tile in turn, and are merged at the item's end.
 // O is rescaled in tensor memory only when a row's maximum has grown by more than 2^8 since its weights were last based on it:
@@ -25,6 +25,9 @@ namespace {
 
 constexpr int ROWS = UMMA_ROWS, COMPUTERS = 2 * ROWS, MAKERS = COMPUTERS / 32 + LOADERS;   // two streams of rows, loading warps,
 constexpr int BLOCK = 32 * (MAKERS + 2);                                                      // a warp a stream that issues products
+// What an item costs, in units (16 trees of 24 nodes 52.1 / 50.4 / 49.0 / 48.1 us at 2 / 4 / 6 / 8, 50.5 at 16; queries, the first scores, the
+// sums' way out), and the shortest run of units that is worth a block.
+constexpr int ITEM_COST = 8, MIN_UNITS = 1;
 constexpr float SLACK = 8.f;                         // log2 of how far weights may exceed 1
 
 // B operand that is contiguous along N: blocks of 64 elements (128-byte swizzle) `lead` bytes apart, groups of 8 rows of K 1024 apart
@@ -140,6 +143,19 @@ __device__ __forceinline__ void tmem_ld_wait_64(uint32_t (&x)[32], uint32_t (&y)
                :
                : "memory");
 }
+// Two fp32 operations an instruction.
+__device__ __forceinline__ uint64_t bits2(float2 v) { return (uint64_t)__float_as_uint(v.y) << 32 | __float_as_uint(v.x); }
+__device__ __forceinline__ float2 float2_of(uint64_t b) { return make_float2(__uint_as_float((uint32_t)b), __uint_as_float((uint32_t)(b >> 32))); }
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(bits2(a)), "l"(bits2(b)), "l"(bits2(c)));
+  return float2_of(d);
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(bits2(a)), "l"(bits2(b)));
+  return float2_of(d);
+}
 // Barriers 1 and 2 are a stream's, 3 is for both, 4 and 5 pass the turn to the first and to the second stream.
 template <int THREADS>
 __device__ __forceinline__ void rows_sync(int id) {
@@ -216,24 +232,26 @@ tree_attention_umma_kernel(const __grid_constant__ CUtensorMap km, const __grid_
     ptx::prefetch_tensormap(&vm);
   }
   ptx::griddep_wait();
-  const long long total = lay_out<BLOCK>(a, TILE_ROWS, seqs, sums, scan_buf);
-  const Line line{seqs, a.pool.sequences, a.cache.heads, group, TILE_ROWS};
-  long long run = (total + gridDim.x - 1) / gridDim.x;
-  if (run < a.min_run) run = a.min_run;
-  const long long u0 = (long long)blockIdx.x * run, u1 = u0 + run < total ? u0 + run : total;
-  if (tid == 0) a.items[blockIdx.x].parts = 0;
-  if (u0 >= u1) return;
-  // Tensor memory before the successor may come: a successor that takes all of it while this block still waits for its share would
-  // wait for this block's end.
+  // Tensor memory, while the others read the batch's lengths.  (Not before the predecessor is done, which may still need its own; and
+  // before the successor may come: one that takes all of it while this block still waits for its share would wait for this block's end.)
   if (warp == MAKERS) {
     ptx::tmem_alloc(ptx::smem_u32(&tmem_slot), S::COLUMNS);
     ptx::tmem_relinquish();
   }
   ptx::tc_fence_before_sync();
-  __syncthreads();
-  ptx::tc_fence_after_sync();
+  const long long total = lay_out<BLOCK>(a, TILE_ROWS, ITEM_COST, seqs, sums, scan_buf);
+  const Line line{seqs, a.pool.sequences, a.cache.heads, group, TILE_ROWS, ITEM_COST};
+  long long run = (total + gridDim.x - 1) / gridDim.x;
+  if (run < MIN_UNITS + ITEM_COST) run = MIN_UNITS + ITEM_COST;
+  const long long u0 = (long long)blockIdx.x * run, u1 = u0 + run < total ? u0 + run : total;
+  if (tid == 0) a.items[blockIdx.x].parts = 0;
+  ptx::tc_fence_after_sync();   // (lay_out ends with the block's barrier)
   ptx::griddep_launch_dependents();
   const uint32_t tmem = tmem_slot;
+  if (u0 >= u1) {
+    if (warp == MAKERS) ptx::tmem_dealloc(tmem, S::COLUMNS);
+    return;
+  }
 
   Place at;
   at.find(line, sums, u0);
@@ -315,27 +333,19 @@ tree_attention_umma_kernel(const __grid_constant__ CUtensorMap km, const __grid_
       const long long first = at.pos - at.unit;   // where the item's units start in the line
       const int r0 = at.tile * TILE_ROWS + (PAIR ? stream * ROWS : 0), rows = at.nodes * group;
       {
-        // 16 bytes a thread and access, eight accesses in flight (one after the other they took 6000 clocks and more)
-        constexpr int LOADING = PAIR ? ROWS : COMPUTERS, STEP = LOADING / PIECES, PASSES = ROWS / STEP, AT_ONCE = PASSES < 8 ? PASSES : 8;
+        // 16 bytes a thread and copy, all of them in flight together (loaded and stored one after the other they took 6000 clocks and more)
+        constexpr int LOADING = PAIR ? ROWS : COMPUTERS, STEP = LOADING / PIECES;
         const int at0 = PAIR ? row_in : tid, piece = at0 % PIECES, row0 = at0 / PIECES;
-        uint8_t* dst = smem + (PAIR ? stream * S::QUERIES : 0) + (piece >> 3) * (ROWS * 128);
+        const uint32_t dst = q_tile + (PAIR ? stream * S::QUERIES : 0) + (piece >> 3) * (ROWS * 128);
+        const uint16_t* src = static_cast<const uint16_t*>(a.io.q) + (int64_t)at.first_row * a.io.q_row_stride + (int64_t)at.head * group * a.io.q_head_stride;
 #pragma unroll
-        for (int p0 = 0; p0 < PASSES; p0 += AT_ONCE) {
-          uint4 x[AT_ONCE];
-#pragma unroll
-          for (int i = 0; i < AT_ONCE; ++i) {
-            const int r = r0 + row0 + (p0 + i) * STEP, t = r / group;
-            x[i] = make_uint4(0, 0, 0, 0);
-            if (r < rows && piece * 8 < dim)
-              x[i] = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.io.q) + (int64_t)(at.first_row + t) * a.io.q_row_stride +
-                                                     (at.head * group + r - t * group) * a.io.q_head_stride + piece * 8);
-          }
-#pragma unroll
-          for (int i = 0; i < AT_ONCE; ++i) {
-            const int row = row0 + (p0 + i) * STEP;
-            *reinterpret_cast<uint4*>(dst + row * 128 + (((piece & 7) ^ (row & 7)) * 16)) = x[i];
-          }
+        for (int i = 0; i < ROWS / STEP; ++i) {
+          const int row = row0 + i * STEP, r = r0 + row, t = r / group;
+          const bool in = r < rows && piece * 8 < dim;
+          cp_async16(dst + row * 128 + (((piece & 7) ^ (row & 7)) * 16),
+                     in ? src + (int64_t)t * a.io.q_row_stride + (r - t * group) * a.io.q_head_stride + piece * 8 : src, in);
         }
+        cp_async_wait_all();
       }
       ptx::fence_proxy_async_smem();
       // (not PAIR: an item of one unit is one stream's alone)
@@ -432,22 +442,23 @@ tree_attention_umma_kernel(const __grid_constant__ CUtensorMap km, const __grid_
           }
         }
         // ---- The streams exponentiate in turn, step by step: left alone they fall into step, share the exponential unit and then both leave
-        // it idle (2060 clocks a step where this takes %%%).
+        // it idle (8 trees of 64 nodes: 124.6 us where this takes 114.5).
         const uint32_t turn = PAIR ? 2 * unit + stream : unit;
         if (turn) rows_sync<COMPUTERS>(4 + (turn & 1));
         // ---- weights (rounded to the 16-bit type: what the tensor cores take; the rounding is unbiased and averages out over positions)
         const float base = m == -INFINITY ? 0.f : m;
         uint32_t p[2][16];   // two weights a word
-        float sum0 = 0.f, sum1 = 0.f;
+        const float2 scale2 = make_float2(a.scale_log2, a.scale_log2), base2 = make_float2(-base, -base);
+        float2 sum2 = make_float2(0.f, 0.f);
 #pragma unroll
         for (int j = 0; j < UNIT; j += 2) {
-          const float x = exp2_approx(fmaf(s[j], a.scale_log2, -base)), y = exp2_approx(fmaf(s[j + 1], a.scale_log2, -base));
-          sum0 += x;
-          sum1 += y;
-          p[j / 32][j / 2 % 16] = pack_pair<F16>(x, y);
+          const float2 y = fma2(make_float2(s[j], s[j + 1]), scale2, base2);
+          const float2 x = make_float2(exp2_approx(y.x), exp2_approx(y.y));
+          sum2 = add2(sum2, x);
+          p[j / 32][j / 2 % 16] = pack_pair<F16>(x.x, x.y);
         }
         rows_arrive<COMPUTERS>(4 + (turn + 1 & 1));
-        l += sum0 + sum1;
+        l += sum2.x + sum2.y;
         ptx::tmem_st_32x32b_x16(s_tmem, p[0]);
         ptx::tmem_st_32x32b_x16(s_tmem + 16, p[1]);
         ptx::tmem_st_wait();
