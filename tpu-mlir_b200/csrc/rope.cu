@@ -4,8 +4,9 @@
 // formed and brought into one turn in 64 bits (at position 131072 a 32-bit product is off by 2^-8 of a radian), and its sine and cosine are
 // taken once for a (row, pair) and shared by all heads of the row through shared memory.
 //
-// What bounds it: HBM for prompts, where every element is read and written once (16 bytes a thread and access); launch and one
-// row's chain position -> angle -> sine -> product for a token.
+// What bounds it: HBM for prompts, where every element is read and written once (16 bytes a thread and access): 195 MB in 34.5 us, 5.65
+// TB/s, 0.86 of the measured rate.  For a token, launch and one row's chain sequence -> length -> page -> write (3.2 us).  Occupancy counts
+// for more than loads in flight a thread: four pieces a thread at once, at 64 registers, took 45 us.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <math.h>
@@ -16,7 +17,7 @@
 namespace b200q {
 namespace {
 
-constexpr int ROPE_THREADS = 256, ROPE_ROWS = 8;   // rows of a block: a warp finds each one's sequence
+constexpr int ROPE_THREADS = 256, ROPE_ROWS = 8;   // most rows of a block: a warp finds each one's sequence
 
 struct RopeArgs {
   b200q_rope_plan plan;
@@ -41,10 +42,20 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
+// Where a pair's cosine and sine stand in a row's table: neighbouring threads take neighbouring pieces, so what they read together stands
+// side by side (two pairs of a piece of eight, one of a piece of four; in the pairs' own order four threads met on a bank).
+template <bool INTERLEAVED, bool WIDE>
+__device__ __forceinline__ int turn_at(int pair, int half) {
+  if (!WIDE) return pair;
+  if (INTERLEAVED) return (pair & 3) * ((half + 3) / 4) + (pair >> 2);
+  return ((pair >> 1 & 3) * (half / 8) + (pair >> 3)) * 2 + (pair & 1);
+}
+__host__ __device__ __forceinline__ int turn_size(int half) { return (half + 3) / 4 * 4; }
+
 // WIDE: 16 bytes at a time (aligned rows and heads; the two halves of a non-interleaved head start on 16 bytes), else one pair.
 template <bool F16, bool INTERLEAVED, bool WIDE>
 __global__ void __launch_bounds__(ROPE_THREADS) rope_kernel(const __grid_constant__ RopeArgs a) {
-  extern __shared__ float2 turn[];                 // [rows_per_block][rotary / 2] (cos, sin), the magnitude in both
+  extern __shared__ __align__(16) float2 turn[];   // [rows_per_block][turn_size] (cos, sin), the magnitude in both
   __shared__ int row_seq[ROPE_ROWS], row_pos[ROPE_ROWS];
   __shared__ int64_t row_entry[ROPE_ROWS];
   const b200q_rope_append& io = a.io;
@@ -80,13 +91,17 @@ __global__ void __launch_bounds__(ROPE_THREADS) rope_kernel(const __grid_constan
     }
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < rows * half; i += ROPE_THREADS) {
-    const int row = i / half, pair = i - row * half;
-    double t = (double)row_pos[row] * a.plan.frequency[pair] * 0.15915494309189533577;   // turns
-    t -= rint(t);
-    float s, c;
-    sincospif(2.f * (float)t, &s, &c);
-    turn[i] = make_float2(c * a.plan.magnitude, s * a.plan.magnitude);
+  if (half) {
+    // a thread keeps to one pair (its frequency is read once) and goes through rows
+    const int at_once = ROPE_THREADS / half, pair = threadIdx.x % half;
+    const double turns_per_position = a.plan.frequency[pair] * 0.15915494309189533577;
+    for (int row = threadIdx.x / half; row < rows && (int)threadIdx.x < at_once * half; row += at_once) {
+      double t = (double)row_pos[row] * turns_per_position;
+      t -= rint(t);
+      float s, c;
+      sincospif(2.f * (float)t, &s, &c);
+      turn[row * turn_size(half) + turn_at<INTERLEAVED, WIDE>(pair, half)] = make_float2(c * a.plan.magnitude, s * a.plan.magnitude);
+    }
   }
   __syncthreads();
 
@@ -95,9 +110,25 @@ __global__ void __launch_bounds__(ROPE_THREADS) rope_kernel(const __grid_constan
   // WIDE and interleaved: eight elements; else: a pair, then the rest by two elements (dim is even)
   const int turned = WIDE ? (INTERLEAVED ? dim / 8 : half / 8) : half;
   const int pieces = turned + (WIDE ? (INTERLEAVED ? 0 : (dim - 2 * half) / 8) : (dim - 2 * half) / 2);
-  for (int i = threadIdx.x; i < rows * heads * pieces; i += ROPE_THREADS) {
-    const int piece = i % pieces, rh = i / pieces, row = rh / heads;
-    int h = h0 + rh - row * heads;
+  // pieces ROPE_THREADS apart: (row, head, piece) goes on by the step's own three digits, with carries (two divisions a piece took longer
+  // than its arithmetic)
+  const int step_piece = ROPE_THREADS % pieces, step_head = ROPE_THREADS / pieces % heads, step_row = ROPE_THREADS / pieces / heads;
+  int piece = threadIdx.x % pieces, head = threadIdx.x / pieces % heads, row = threadIdx.x / pieces / heads;
+  auto go_on = [&]() {
+    piece += step_piece;
+    head += step_head;
+    row += step_row;
+    if (piece >= pieces) {
+      piece -= pieces;
+      ++head;
+    }
+    if (head >= heads) {
+      head -= heads;
+      ++row;
+    }
+  };
+  for (; row < rows; go_on()) {
+    int h = h0 + head;
     if (row_seq[row] < 0) continue;
     const int64_t r = r0 + row;
     const uint16_t* x;
@@ -115,7 +146,7 @@ __global__ void __launch_bounds__(ROPE_THREADS) rope_kernel(const __grid_constan
                 : static_cast<const uint16_t*>(io.v) + r * io.v_row_stride + h * io.v_head_stride;
       y = static_cast<uint16_t*>(turns ? a.cache.k : a.cache.v) + io.layer * a.cache.layer_stride + row_entry[row] + h * a.cache.head_stride;
     }
-    const float2* t = turn + row * half;
+    const float2* t = turn + row * turn_size(half);
     if (WIDE && INTERLEAVED) {
       uint4 v = *reinterpret_cast<const uint4*>(x + piece * 8);
       uint32_t w[4] = {v.x, v.y, v.z, v.w};
@@ -123,7 +154,7 @@ __global__ void __launch_bounds__(ROPE_THREADS) rope_kernel(const __grid_constan
       for (int j = 0; j < 4; ++j) {
         const int pair = piece * 4 + j;
         if (turns && pair < half) {
-          const float2 cs = t[pair];
+          const float2 cs = t[turn_at<true, true>(pair, half)];
           const float p = to_f32<F16>(w[j] & 0xffffu), q = to_f32<F16>(w[j] >> 16);
           w[j] = pack2<F16>(p * cs.x - q * cs.y, q * cs.x + p * cs.y);
         }
@@ -136,7 +167,8 @@ __global__ void __launch_bounds__(ROPE_THREADS) rope_kernel(const __grid_constan
         if (turns) {
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            const float2 c0 = t[piece * 8 + 2 * j], c1 = t[piece * 8 + 2 * j + 1];
+            const float4 cs = *reinterpret_cast<const float4*>(t + turn_at<false, true>(piece * 8 + 2 * j, half));   // two pairs
+            const float2 c0 = make_float2(cs.x, cs.y), c1 = make_float2(cs.z, cs.w);
             const float p0 = to_f32<F16>(wp[j] & 0xffffu), p1 = to_f32<F16>(wp[j] >> 16);
             const float q0 = to_f32<F16>(wq[j] & 0xffffu), q1 = to_f32<F16>(wq[j] >> 16);
             wp[j] = pack2<F16>(p0 * c0.x - q0 * c0.y, p1 * c1.x - q1 * c1.y);
@@ -178,9 +210,11 @@ int launch_rope(RopeArgs& a, bool f16, bool wide, int sms, cudaStream_t s) {
   const int half = a.plan.rotary_dim / 2;
   wide = wide && a.plan.head_dim % 8 == 0 && (interleaved || half % 8 == 0);
   const int pieces = wide ? (interleaved ? a.plan.head_dim / 8 : half / 8 + (a.plan.head_dim - 2 * half) / 8) : a.plan.head_dim / 2;
-  // As many rows a block as leave four blocks an SM (sines are taken once for a row of a block); with fewer rows than that the
-  // heads are spread over blocks until a thread has one piece, and every block takes the row's sines for itself.
-  int rows = ROPE_ROWS;
+  // Rows of a block: three pieces a thread (8000 rows of 48 heads: 35 us with two rows, 37 with four, 41 with eight, 39 with one: sines are
+  // taken once for a row of a block, but short blocks hide each other's start), fewer where that leaves no four blocks an SM.  With still
+  // fewer rows the heads are spread over blocks until a thread has one piece, and every block takes the row's sines for itself.
+  int rows = 1;
+  while (rows < ROPE_ROWS && (int64_t)rows * a.heads * pieces < 3 * ROPE_THREADS) rows *= 2;
   while (rows > 1 && (a.io.rows + rows - 1) / rows < 4LL * sms) rows /= 2;
   int splits = 1;
   while (a.io.rows * splits < 4LL * sms && (int64_t)rows * ((a.heads + splits - 1) / splits) * pieces > ROPE_THREADS && splits < a.heads) splits *= 2;
@@ -189,7 +223,7 @@ int launch_rope(RopeArgs& a, bool f16, bool wide, int sms, cudaStream_t s) {
   const int64_t blocks = (a.io.rows + rows - 1) / rows;
   if (blocks > 0x7fffffffLL) return set_error(B200Q_ERR_UNSUPPORTED, "rope: too many rows");
   const dim3 grid((unsigned)blocks, (a.heads + a.heads_per_block - 1) / a.heads_per_block);
-  const size_t smem = (size_t)rows * half * sizeof(float2);
+  const size_t smem = (size_t)rows * turn_size(half) * sizeof(float2);
 #define B200Q_ROPE(F, I, W) return launch_dependent(rope_kernel<F, I, W>, grid, dim3(ROPE_THREADS), smem, s, a)
   if (f16) {
     if (interleaved) { if (wide) B200Q_ROPE(true, true, true); else B200Q_ROPE(true, true, false); }
