@@ -78,24 +78,27 @@ int sm_count(int device) {
 
 namespace {
 
+// The planning kernels are one block, compiled for two an SM (32 registers): it fits beside what the kernel before it still runs, and
+// starts while that drains (at 60 registers the fork of 16 beams took 4 us more).
 constexpr int PLAN_THREADS = 1024;
 
-// Inclusive sum over the block's threads, one value each; every thread also gets the total.  buf: 33 words of shared memory.
-__device__ __forceinline__ long long block_scan(long long v, long long* buf, long long* total) {
+// Inclusive sum over the block's threads, one value each; every thread also gets the total.  buf: 32 of shared memory.
+template <typename T>
+__device__ __forceinline__ T block_scan(T v, T* buf, T* total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
-    const long long o = __shfl_up_sync(0xffffffffu, v, d);
+    const T o = __shfl_up_sync(0xffffffffu, v, d);
     if (lane >= d) v += o;
   }
   __syncthreads();   // buf may still be read from the scan before
   if (lane == 31) buf[warp] = v;
   __syncthreads();
   if (warp == 0) {
-    long long w = lane < (int)(blockDim.x >> 5) ? buf[lane] : 0;
+    T w = buf[lane];
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
-      const long long o = __shfl_up_sync(0xffffffffu, w, d);
+      const T o = __shfl_up_sync(0xffffffffu, w, d);
       if (lane >= d) w += o;
     }
     buf[lane] = w;
@@ -105,95 +108,88 @@ __device__ __forceinline__ long long block_scan(long long v, long long* buf, lon
   return v + (warp ? buf[warp - 1] : 0);
 }
 
-// The `need` lowest free pages, in order: give(rank, page) is called once for every rank below `need`, by some thread.  Nothing is
-// called and false returned when there are fewer.  All threads of a block of PLAN_THREADS call it; bitmap: a word for 32 pages.
+// Four pages' bits where sixteen bytes cannot be read at once.
+__device__ __noinline__ uint32_t free_one_by_one(const int32_t* refcount, int at, int pages) {
+  uint32_t w = 0;
+#pragma unroll 1
+  for (int e = 0; e < 4 && at + e < pages; ++e) w |= (uint32_t)(refcount[at + e] == 0) << e;
+  return w;
+}
+
+// The `need` lowest free pages, in order: give(first, rank, page, mine) is called by whole warps, `mine` once for every rank below `need`;
+// `first` is the rank of the warp's first free page.  Nothing is called and false returned when there are fewer.  All threads of a block of PLAN_THREADS call it; bitmap: a word for 32 pages.
 //
-// Free pages become bits (a lane looks at four counts, eight lanes' nibbles make a word), 32768 pages a step so that all loads of a
-// step are in flight, and the steps end once enough are found; ranks are the sums of the bits before, by a scan over the threads'
-// runs of words.
+// Free pages become bits (a lane looks at four counts, eight lanes' nibbles make a word), 16384 pages a step so that all loads of a
+// step are in flight, and the steps end once enough are found.  Then, 1024 words a step, ranks are the sums of the bits before (a scan),
+// and the words are dealt out to the warps one by one, a bit a lane: free pages stand together, and a warp that had a run of them to
+// itself took 17 us for 5000.
 template <typename Give>
-__device__ bool lowest_free(const int32_t* refcount, int pages, long long need, uint32_t* bitmap, long long* buf, Give give) {
+__device__ bool lowest_free(const int32_t* refcount, int pages, long long need, uint32_t* bitmap, int* ranks, int* buf, Give give) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = PLAN_THREADS / 32;
   const bool wide = (reinterpret_cast<uintptr_t>(refcount) & 15) == 0;
-  constexpr int PER_WARP = 1024;                   // pages of a step that a warp looks at, 128 at a time
-  int seen = 0;                                    // pages whose bits are set up (a multiple of 128 but for the last)
-  long long found = 0;
+  constexpr int PER_WARP = 512;                    // pages of a step that a warp looks at, 128 at a time
+  int seen = 0, found = 0;                         // pages whose bits are set up; how many of them are free
+  if (threadIdx.x == 0) ranks[0] = 0;
+  __syncthreads();
   while (seen < pages && found < need) {
-    const int first = seen + warp * PER_WARP;
+    const int first = seen + warp * PER_WARP + lane * 4;
     int4 c[PER_WARP / 128];
 #pragma unroll
-    for (int i = 0; i < PER_WARP / 128; ++i) {
-      const int p = first + i * 128 + lane * 4;
-      c[i] = make_int4(1, 1, 1, 1);
-      if (wide && p + 4 <= pages) {
-        c[i] = *reinterpret_cast<const int4*>(refcount + p);
-      } else {
-        if (p < pages) c[i].x = refcount[p];
-        if (p + 1 < pages) c[i].y = refcount[p + 1];
-        if (p + 2 < pages) c[i].z = refcount[p + 2];
-        if (p + 3 < pages) c[i].w = refcount[p + 3];
-      }
-    }
+    for (int i = 0; i < PER_WARP / 128; ++i)
+      c[i] = wide && first + i * 128 + 4 <= pages ? *reinterpret_cast<const int4*>(refcount + first + i * 128) : make_int4(1, 1, 1, 1);
     int mine = 0;
 #pragma unroll
     for (int i = 0; i < PER_WARP / 128; ++i) {
+      const int at = first + i * 128;
       uint32_t w = (uint32_t)(c[i].x == 0) | (uint32_t)(c[i].y == 0) << 1 | (uint32_t)(c[i].z == 0) << 2 | (uint32_t)(c[i].w == 0) << 3;
+      if (at < pages && !(wide && at + 4 <= pages)) w = free_one_by_one(refcount, at, pages);
       w <<= 4 * (lane & 7);
       w |= __shfl_xor_sync(0xffffffffu, w, 1);
       w |= __shfl_xor_sync(0xffffffffu, w, 2);
       w |= __shfl_xor_sync(0xffffffffu, w, 4);
-      const int at = first + i * 128 + (lane >> 3) * 32;
       if ((lane & 7) == 0 && at < pages) {
         bitmap[at >> 5] = w;
         mine += __popc(w);
       }
     }
-    long long total;
-    block_scan(mine, buf, &total);
-    found += total;
+    mine = __reduce_add_sync(0xffffffffu, mine);
+    if (lane == 0 && mine) atomicAdd(&ranks[0], mine);
+    __syncthreads();
+    found = ranks[0];
+    __syncthreads();   // (before the next step adds to it)
     seen = seen + warps * PER_WARP < pages ? seen + warps * PER_WARP : pages;
   }
   if (found < need) return false;
-  const int words = (seen + 31) >> 5, each = (words + PLAN_THREADS - 1) / PLAN_THREADS;
-  const int w0 = threadIdx.x * each;
-  int mine = 0;
-  for (int i = 0; i < each; ++i)
-    if (w0 + i < words) mine += __popc(bitmap[w0 + i]);
-  long long total;
-  long long rank = block_scan(mine, buf, &total) - mine;
-  // a warp goes through its lanes' words together, a bit a lane: neighbouring ranks are handed out by neighbouring lanes
-  for (int i = 0; i < each; ++i) {
-    const uint32_t w = w0 + i < words ? bitmap[w0 + i] : 0u;
-    uint32_t some = __ballot_sync(0xffffffffu, w != 0u && rank < need);
-    while (some) {
-      const int src = __ffs(some) - 1;
-      some &= some - 1;
-      const uint32_t bits = __shfl_sync(0xffffffffu, w, src);
-      const long long base = __shfl_sync(0xffffffffu, rank, src);
-      const int word = __shfl_sync(0xffffffffu, w0, src) + i;
-      const long long r = base + __popc(bits & ((1u << lane) - 1u));
-      if ((bits >> lane & 1u) && r < need) give(r, word * 32 + lane);
+  const int words = (seen + 31) >> 5;
+  long long before = 0;
+  for (int w0 = 0; w0 < words && before < need; w0 += PLAN_THREADS) {
+    const int mine = w0 + (int)threadIdx.x < words ? __popc(bitmap[w0 + threadIdx.x]) : 0;
+    int total;
+    const int upto = block_scan(mine, buf, &total);
+    ranks[threadIdx.x] = upto - mine;
+    __syncthreads();
+#pragma unroll 1
+    for (int k = warp; k < PLAN_THREADS && w0 + k < words && before + ranks[k] < need; k += warps) {
+      const uint32_t bits = bitmap[w0 + k];
+      const long long first = before + ranks[k], r = first + __popc(bits & ((1u << lane) - 1u));
+      give(first, r, (w0 + k) * 32 + lane, (bits >> lane & 1u) && r < need);
     }
-    rank += __popc(w);
+    before += total;
   }
   return true;
 }
 
-// The first of n ascending sums that is above `rank`.
-__device__ __forceinline__ int owner(const long long* sums, int n, long long rank) {
-  int lo = 0, hi = n - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    if (sums[mid] > rank) hi = mid;
-    else lo = mid + 1;
-  }
-  return lo;
+// The first of PLAN_THREADS ascending sums that is above `rank`, found by a warp: which 32 of them, then which of those.
+__device__ __forceinline__ int owner(const long long* sums, long long rank) {
+  const int lane = threadIdx.x & 31;
+  const int group = __popc(__ballot_sync(0xffffffffu, sums[lane * 32 + 31] <= rank));
+  return group * 32 + __popc(__ballot_sync(0xffffffffu, sums[(group & 31) * 32 + lane] <= rank));
 }
 
-__global__ void __launch_bounds__(PLAN_THREADS) reserve_kernel(b200q_kv_pool pool, const int32_t* __restrict__ extra, int32_t* status) {
+__global__ void __launch_bounds__(PLAN_THREADS, 2) reserve_kernel(b200q_kv_pool pool, const int32_t* __restrict__ extra, int32_t* status) {
   extern __shared__ uint32_t bitmap[];
-  __shared__ long long buf[33], sums[KV_MAX_SEQUENCES];
-  __shared__ int base[KV_MAX_SEQUENCES];
+  __shared__ long long wide_buf[32], sums[KV_MAX_SEQUENCES];
+  __shared__ int base[KV_MAX_SEQUENCES], ranks[PLAN_THREADS], buf[32];
   const int s = threadIdx.x;
   ptx::griddep_launch_dependents();
   ptx::griddep_wait();
@@ -208,7 +204,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) reserve_kernel(b200q_kv_pool poo
     narrow = want > pool.table_width;
   }
   long long total;
-  const long long upto = block_scan(need, buf, &total);
+  const long long upto = block_scan(need, wide_buf, &total);
   sums[s] = upto;
   base[s] = held - (int)(upto - need);   // column of rank r: base + r
   if (__syncthreads_or(narrow)) {
@@ -216,8 +212,10 @@ __global__ void __launch_bounds__(PLAN_THREADS) reserve_kernel(b200q_kv_pool poo
     return;
   }
   if (total == 0) return;
-  const bool ok = lowest_free(pool.refcount, pool.pages, total, bitmap, buf, [&](long long r, int page) {
-    const int t = owner(sums, pool.sequences, r);
+  const bool ok = lowest_free(pool.refcount, pool.pages, total, bitmap, ranks, buf, [&](long long first, long long r, int page, bool mine) {
+    int t = owner(sums, first);
+    if (!mine) return;
+    while (sums[t] <= r) ++t;
     pool.table[t * pool.table_stride + base[t] + (int)r] = page;
     pool.refcount[page] = 1;
   });
@@ -256,10 +254,9 @@ __device__ __forceinline__ ForkScratch fork_scratch(int32_t* w, int n) {
   return {w, w + 1, w + 2, w + 2 + n, w + 2 + 2 * n, w + 2 + 3 * n, w + 2 + 4 * n};
 }
 
-__global__ void __launch_bounds__(PLAN_THREADS) fork_plan_kernel(b200q_kv_pool pool, const int32_t* __restrict__ parent, int32_t* status) {
+__global__ void __launch_bounds__(PLAN_THREADS, 2) fork_plan_kernel(b200q_kv_pool pool, const int32_t* __restrict__ parent, int32_t* status) {
   extern __shared__ uint32_t bitmap[];
-  __shared__ long long buf[33];
-  __shared__ int list[KV_MAX_SEQUENCES], lengths[KV_MAX_SEQUENCES];
+  __shared__ int buf[32], list[KV_MAX_SEQUENCES], lengths[KV_MAX_SEQUENCES], ranks[PLAN_THREADS];
   const int s = threadIdx.x, n = pool.sequences;
   const ForkScratch f = fork_scratch(pool.scratch, n);
   ptx::griddep_launch_dependents();
@@ -269,8 +266,8 @@ __global__ void __launch_bounds__(PLAN_THREADS) fork_plan_kernel(b200q_kv_pool p
   const int p = s < n ? parent[s] : -1;
   const bool child = p >= 0 && p < n && p != s;
   const int count = child ? lengths[p] : 0, ragged = count % pool.page_size != 0;
-  long long total;
-  const long long rank = block_scan(ragged, buf, &total) - ragged;
+  int total;
+  const int rank = block_scan(ragged, buf, &total) - ragged;
   if (ragged) list[rank] = s;
   if (s < n) {
     f.length[s] = lengths[s];
@@ -279,12 +276,14 @@ __global__ void __launch_bounds__(PLAN_THREADS) fork_plan_kernel(b200q_kv_pool p
     f.source[s] = ragged ? kv_page(pool, p, count) : -1;
   }
   if (s == 0) {
-    *f.ragged = (int)total;
+    *f.ragged = total;
     *f.go = 1;
   }
   __syncthreads();
   if (s < total) f.list[s] = list[s];
-  const bool ok = total == 0 || lowest_free(pool.refcount, pool.pages, total, bitmap, buf, [&](long long r, int page) { f.page[list[r]] = page; });
+  const bool ok = total == 0 || lowest_free(pool.refcount, pool.pages, total, bitmap, ranks, buf, [&](long long, long long r, int page, bool mine) {
+    if (mine) f.page[list[r]] = page;
+  });
   if (!ok) {
     if (s == 0) {
       *f.go = 0;
@@ -298,12 +297,12 @@ __global__ void __launch_bounds__(PLAN_THREADS) fork_plan_kernel(b200q_kv_pool p
   }
 }
 
-constexpr int FORK_THREADS = 256;
-constexpr int FORK_TILE = 8192;   // table entries of a tile: at least 8 columns of 1024 sequences
+constexpr int FORK_THREADS = 256, FORK_AT_ONCE = 4, FORK_PER_SM = 4;
+constexpr int FORK_TILE = 2048;   // table entries of a tile: at least 2 columns of 1024 sequences
 
 // Blocks below `table_blocks` take the tables, a run of columns each: all sequences' entries of these columns are read before the
 // first is written, so children may be parents.  The other blocks copy ragged pages, a (child, layer, keys or values) at a time.
-__global__ void __launch_bounds__(FORK_THREADS)
+__global__ void __launch_bounds__(FORK_THREADS, FORK_PER_SM)
 fork_kernel(b200q_kv_cache cache, b200q_kv_pool pool, const int32_t* __restrict__ parent, int table_blocks, int columns) {
   __shared__ int32_t old[FORK_TILE];
   const int n = pool.sequences;
@@ -345,45 +344,57 @@ fork_kernel(b200q_kv_cache cache, b200q_kv_pool pool, const int32_t* __restrict_
     if (from < 0) continue;
     const int slots = f.length[parent[s]] % pool.page_size;
     uint16_t* base = static_cast<uint16_t*>(part & 1 ? cache.v : cache.k) + (part >> 1) * cache.layer_stride;
-    const int inner = slots_outside ? cache.heads : slots;
-    for (int i = threadIdx.x; i < slots * cache.heads * chunks; i += FORK_THREADS) {
-      const int d = i % chunks, row = i / chunks, a = row / inner, b = row % inner;
-      const int64_t at = (slots_outside ? a * cache.slot_stride + b * cache.head_stride : b * cache.slot_stride + a * cache.head_stride) + d * 8;
-      *reinterpret_cast<uint4*>(base + to * cache.page_stride + at) = *reinterpret_cast<const uint4*>(base + from * cache.page_stride + at);
+    const int inner = slots_outside ? cache.heads : slots, count = slots * cache.heads * chunks;
+    const uint16_t* src = base + from * cache.page_stride;
+    uint16_t* dst = base + to * cache.page_stride;
+    for (int i0 = threadIdx.x; i0 < count; i0 += FORK_AT_ONCE * FORK_THREADS) {
+      uint4 v[FORK_AT_ONCE];
+      int64_t at[FORK_AT_ONCE];
+#pragma unroll
+      for (int j = 0; j < FORK_AT_ONCE; ++j) {
+        const int i = i0 + j * FORK_THREADS, row = i / chunks, x = row / inner, y = row - x * inner;
+        at[j] = (slots_outside ? x * cache.slot_stride + y * cache.head_stride : y * cache.slot_stride + x * cache.head_stride) + (i - row * chunks) * 8;
+        if (i < count) v[j] = *reinterpret_cast<const uint4*>(src + at[j]);
+      }
+#pragma unroll
+      for (int j = 0; j < FORK_AT_ONCE; ++j)
+        if (i0 + j * FORK_THREADS < count) *reinterpret_cast<uint4*>(dst + at[j]) = v[j];
     }
   }
 }
 
-// ---- compact.  A block takes a (sequence, layer, keys or values); a thread takes 16 bytes of a head and walks along the path.
+// ---- compact.  A block takes some (layer, keys or values) of a sequence, whose places it looks up once; a thread takes 16 bytes of a head
+// and walks along the path.
 // Entry i is moved to place i <= path[i], and no later source lies at or before place i (the path ascends), so loads may run ahead of
 // stores but not the other way: eight loads, then their stores.
 constexpr int COMPACT_THREADS = 128, PATH_MOST = 1024, COMPACT_AHEAD = 8;
 
 __global__ void __launch_bounds__(COMPACT_THREADS)
 compact_kernel(b200q_kv_cache cache, b200q_kv_pool pool, const int32_t* __restrict__ path, int64_t path_stride, int path_width,
-               const int32_t* __restrict__ path_length, int32_t* __restrict__ length_out) {
+               const int32_t* __restrict__ path_length, int32_t* __restrict__ length_out, int parts_each) {
   __shared__ int64_t from[PATH_MOST], to[PATH_MOST];
   __shared__ int good;
   const int parts = 2 * cache.layers, chunks = cache.head_dim / 8;
   ptx::griddep_launch_dependents();
   ptx::griddep_wait();
-  for (int item = blockIdx.x; item < pool.sequences * parts; item += gridDim.x) {
-    const int s = item / parts, part = item % parts, length = kv_length(pool, s);
-    int n = path_length[s];
-    n = n < 0 ? 0 : n < path_width ? n : path_width;
-    if (threadIdx.x == 0) good = n;
-    __syncthreads();
-    for (int i = threadIdx.x; i < n; i += COMPACT_THREADS) {
-      const int32_t* row = path + s * path_stride;
-      const int node = row[i], before = i ? row[i - 1] : -1;
-      const bool in = node > before && node >= i && (int64_t)length + node <= 0x7fffffffLL;
-      from[i] = in ? kv_entry(cache, pool, s, length + node) : -1;
-      to[i] = in ? kv_entry(cache, pool, s, length + i) : -1;
-      if (from[i] < 0 || to[i] < 0) atomicMin(&good, i);
-    }
-    __syncthreads();
-    n = good;
-    if (part == 0 && threadIdx.x == 0) length_out[s] = length + n;
+  const int blocks_each = (parts + parts_each - 1) / parts_each, s = blockIdx.x / blocks_each, part0 = blockIdx.x % blocks_each * parts_each;
+  const int length = kv_length(pool, s);
+  int n = path_length[s];
+  n = n < 0 ? 0 : n < path_width ? n : path_width;
+  if (threadIdx.x == 0) good = n;
+  __syncthreads();
+  for (int i = threadIdx.x; i < n; i += COMPACT_THREADS) {
+    const int32_t* row = path + s * path_stride;
+    const int node = row[i], before = i ? row[i - 1] : -1;
+    const bool in = node > before && node >= i && (int64_t)length + node <= 0x7fffffffLL;
+    from[i] = in ? kv_entry(cache, pool, s, length + node) : -1;
+    to[i] = in ? kv_entry(cache, pool, s, length + i) : -1;
+    if (from[i] < 0 || to[i] < 0) atomicMin(&good, i);
+  }
+  __syncthreads();
+  n = good;
+  if (part0 == 0 && threadIdx.x == 0) length_out[s] = length + n;
+  for (int part = part0; part < part0 + parts_each && part < parts; ++part) {
     uint16_t* base = static_cast<uint16_t*>(part & 1 ? cache.v : cache.k) + (part >> 1) * cache.layer_stride;
     for (int c = threadIdx.x; c < cache.heads * chunks; c += COMPACT_THREADS) {
       uint16_t* p = base + (c / chunks) * cache.head_stride + (c % chunks) * 8;
@@ -397,7 +408,6 @@ compact_kernel(b200q_kv_cache cache, b200q_kv_pool pool, const int32_t* __restri
           if (i0 + j < n && from[i0 + j] != to[i0 + j]) *reinterpret_cast<uint4*>(p + to[i0 + j]) = v[j];
       }
     }
-    __syncthreads();   // from, to and good are the next item's
   }
 }
 
@@ -466,12 +476,12 @@ int b200q_kv_fork_dev(const b200q_kv_cache* cache, const b200q_kv_pool* pool, co
   size_t bytes;
   B200Q_TRY(bitmap_bytes((const void*)fork_plan_kernel, pool->pages, &bytes));
   B200Q_TRY(launch_dependent(fork_plan_kernel, dim3(1), dim3(PLAN_THREADS), bytes, s, *pool, parent, status));
-  // 32 columns a tile where they fit, at least 8
+  // 32 columns a tile where they fit, at least 2
   int columns = FORK_TILE / pool->sequences;
   columns = columns > 32 ? 32 : columns;
   const int tiles = ceil_div(pool->table_width, columns), table_blocks = tiles < sms ? tiles : sms;
   const int64_t copies = (int64_t)pool->sequences * 2 * cache->layers;
-  const int copy_blocks = (int)(copies < 4 * sms ? copies : 4 * sms);
+  const int copy_blocks = (int)(copies < FORK_PER_SM * sms ? copies : FORK_PER_SM * sms);
   return launch_dependent(fork_kernel, dim3(table_blocks + copy_blocks), dim3(FORK_THREADS), 0, s, *cache, *pool, parent, table_blocks, columns);
 }
 
@@ -488,10 +498,14 @@ int b200q_kv_compact_dev(const b200q_kv_cache* cache, const b200q_kv_pool* pool,
   OnDeviceOf dev("kv_compact", pool->table);
   B200Q_TRY(dev.rc);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  // (a block with nothing to move is gone in a microsecond: the grid only has to keep the memory busy)
-  const int64_t items = (int64_t)pool->sequences * 2 * cache->layers;
-  B200Q_TRY(launch_dependent(compact_kernel, dim3((unsigned)(items < 65536 ? items : 65536)), dim3(COMPACT_THREADS), 0, s, *cache, *pool, path,
-                             path_stride, path_width, path_length, in_place ? pool->scratch : length_out));
+  const int sms = sm_count(dev.device);
+  if (sms < 0) return sms;
+  // all blocks at once where that is possible: sixteen fit an SM
+  const int parts = 2 * cache->layers;
+  const int64_t items = (int64_t)pool->sequences * parts;
+  const int parts_each = (int)((items + 16 * sms - 1) / (16 * sms)), each = parts_each < parts ? parts_each : parts;
+  B200Q_TRY(launch_dependent(compact_kernel, dim3((unsigned)(pool->sequences * ((parts + each - 1) / each))), dim3(COMPACT_THREADS), 0, s, *cache, *pool,
+                             path, path_stride, path_width, path_length, in_place ? pool->scratch : length_out, each));
   if (in_place) B200Q_TRY(launch_dependent(lengths_kernel, dim3(1), dim3(KV_MAX_SEQUENCES), 0, s, pool->scratch, pool->length, pool->sequences));
   return B200Q_OK;
 }
