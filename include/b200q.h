@@ -605,8 +605,8 @@ int b200q_top_distance_f32_dev(const float *x, const float *ref, int64_t count, 
  * structs is a DEVICE pointer of one device, the structs themselves are read during the call; calls are asynchronous on
  * `stream`, allocate nothing and never synchronise, so they can be captured.  They run on the device that holds the pool's
  * tables (or x), whichever device is current.  `stream` belongs to that device, or is NULL for its legacy default stream.
- * What only the device sees (lengths, page numbers, row starts, paths) is never trusted with an address: a page number
- * outside the pool or a position past the table is not read or written, as each function says. */
+ * What only the device sees (lengths, page numbers, row starts, paths) is never trusted with an address: a position
+ * without a page in the pool is not read or written, as each function says. */
 
 /* Keys and values: element (layer, page, slot, head, d) of either lies at layer * layer_stride + page * page_stride +
  * slot * slot_stride + head * head_stride + d, in elements; any order of the dimensions.  k, v 16-byte aligned, strides
@@ -619,8 +619,8 @@ typedef struct {
 } b200q_kv_cache;
 
 /* Which pages a sequence holds.  Position p of sequence s lies in page table[s * table_stride + p / page_size], slot
- * p % page_size, for p / page_size < table_width; entries past held[s] are not meaningful (-1 where a call here cleared
- * them).  length[s] positions are committed; refcount[p] sequences hold page p, 0 means free.  A new pool is refcount = 0,
+ * p % page_size, for p / page_size < held[s] <= table_width; it has no page past that, or where the table's entry is none of the
+ * pool's.  Entries past held[s] are not read (-1 where a call here cleared them).  length[s] positions are committed; refcount[p] sequences hold page p, 0 means free.  A new pool is refcount = 0,
  * held = 0, length = 0.  `scratch` is working space of at least b200q_kv_scratch_words(sequences) words whose contents need not be
  * kept: calls that use it (fork, compact) and can overlap need pools with scratch of their own.  Limits: 1024 sequences,
  * 1048576 pages, table_width * page_size below 2^31. */
@@ -642,7 +642,7 @@ int b200q_kv_free_dev(const b200q_kv_pool *pool, const int32_t *which, void *str
 /* Every sequence s with a parent[s] other than s in [0, sequences) becomes what that sequence was BEFORE the call (beams
  * reordered in one call; swaps and several children of one parent included); other values of parent leave s alone.  Full
  * pages are shared; the filled slots of a ragged last page are copied in every layer into a page of the child's own (the
- * lowest-numbered pages free before the call, in the order of the sequences); pages held past the parent's length are not passed on;
+ * lowest-numbered pages free before the call, in the order of the sequences); pages held past the parent's length are not passed on, nor positions without a page;
  * what s held is given back after that.  When the free pages do not suffice nothing changes and *status (optional) becomes 1. */
 int b200q_kv_fork_dev(const b200q_kv_cache *cache, const b200q_kv_pool *pool, const int32_t *parent, int32_t *status, void *stream);
 /* Keeps the accepted path of a tree of drafted tokens whose entries stand at positions length[s] + node: for i below
@@ -708,7 +708,7 @@ int b200q_rope_append_dev(const b200q_rope_plan *plan, const b200q_kv_cache *cac
  * chain, m <= n (one row a sequence: plain decoding).
  *   out = sum_j w_j v_j / sum_j w_j,  w_j = exp(scale * (q . k_j) - max)
  * A row that sees nothing (and one whose scores are all -inf) becomes zeros; what a row does not see does not touch it, infinities
- * and NaN included.  Positions whose page is not in the pool are not seen.  Rows outside every sequence stay as they are.  Products and sums in
+ * and NaN included.  Positions without a page are not seen.  Rows outside every sequence stay as they are.  Products and sums in
  * fp32, the weights rounded to the 16-bit type before the second product.  q, out 16-byte aligned with strides of multiples of 8
  * elements; scale positive.  workspace: b200q_tree_attention_workspace bytes, 16-byte aligned, contents irrelevant before and after;
  * calls that can overlap (two captured graphs replayed at a time among them) need one each. */

@@ -77,7 +77,7 @@ class Pool:
     def place(self, s, pos):
         """(page, slot) or None."""
         j = pos // self.page_size
-        if pos < 0 or j >= self.width or not 0 <= self.table[s][j] < len(self.refcount):
+        if pos < 0 or j >= min(self.held[s], self.width) or not 0 <= self.table[s][j] < len(self.refcount):
             return None
         return self.table[s][j], pos % self.page_size
 

@@ -62,7 +62,9 @@ BAD_POOLS = [(dict(table=None), L.ERR_INVALID, b"null"), (dict(length=None), L.E
 BAD_CACHES = [(dict(k=None), L.ERR_INVALID, b"null"), (dict(v=None), L.ERR_INVALID, b"null"), (dict(v=FAKE + 8), L.ERR_INVALID, b"aligned"),
               (dict(dtype=L.DT_F32), L.ERR_UNSUPPORTED, b"bf16"), (dict(layers=0), L.ERR_INVALID, b"shape"), (dict(heads=0), L.ERR_INVALID, b"shape"),
               (dict(head_dim=0), L.ERR_INVALID, b"shape"), (dict(head_dim=60), L.ERR_UNSUPPORTED, b"head_dim"), (dict(head_dim=264), L.ERR_UNSUPPORTED, b"head_dim"),
-              (dict(slot_stride=132), L.ERR_INVALID, b"strides"), (dict(page_stride=1), L.ERR_INVALID, b"strides")]
+              (dict(slot_stride=132), L.ERR_INVALID, b"strides"), (dict(page_stride=1), L.ERR_INVALID, b"strides"),
+              (dict(head_stride=0), L.ERR_INVALID, b"positive"), (dict(slot_stride=-128), L.ERR_INVALID, b"positive"), (dict(layer_stride=-8), L.ERR_INVALID, b"positive"),
+              (dict(page_stride=1 << 38), L.ERR_INVALID, b"positive")]
 
 
 def calls(lib, c, p, a=None, r=None, pl=None):

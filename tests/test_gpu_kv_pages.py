@@ -5,7 +5,8 @@ import pytest
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
 
-from decode_util import Cache, i32  # noqa: E402
+from decode_model import Pool, attention  # noqa: E402
+from decode_util import Cache, f64, i32, rope_plan, words  # noqa: E402
 
 
 def filled(c, lengths):
@@ -215,3 +216,103 @@ def test_a_captured_step_on_another_stream():
         c.model.free([0, 0, 0, 1])
         c.same_state()
         assert torch.equal(c.k, k) and c.status.item() == 0
+
+
+def test_counts_off_sixteen_bytes_and_a_pool_that_fills_the_default_shared_memory():
+    c = Cache(sequences=2, width=40000, pages=262144, page_size=8, heads=1, dim=8)
+    c.reserve([300000, 17])
+    assert c.model.reserve([300000, 17]) == 0
+    c.same_state()
+    back = torch.zeros(70, dtype=torch.int32, device="cuda")
+    for shift in (1, 2, 3):
+        c = Cache(sequences=2, width=30, pages=61, page_size=4, heads=1, dim=8)
+        back.zero_()
+        back[:shift] = back[shift + 61:] = -9
+        c.refcount = back[shift:shift + 61]
+        for extra in ([50, 70], [80, 90], [400, 1]):
+            c.reserve(extra)
+            c.model.reserve(extra)
+            c.same_state()
+        assert (back[:shift] == -9).all() and (back[shift + 61:] == -9).all()
+
+
+def test_without_a_status_word():
+    import ctypes as C
+
+    import tpu_mlir_b200._lib as L
+    c = Cache(sequences=2, width=2, pages=3, page_size=4, heads=1, dim=8)
+    lib = L.lib()
+    for extra in ([9, 0], [8, 8], [8, 1]):       # too wide, too many, just right
+        e = i32(extra)
+        L.check(lib.b200q_kv_reserve_dev(C.byref(c.pool()), e.data_ptr(), None, None))
+        c.model.reserve(extra)
+        c.same_state()
+    c.model.length = [7, 0]
+    c.up()
+    p = i32([0, 0])
+    L.check(lib.b200q_kv_fork_dev(C.byref(c.cache()), C.byref(c.pool()), p.data_ptr(), None, None))    # no page is free
+    c.same_state()
+
+
+def test_entries_past_the_held_pages_are_not_looked_at():
+    """A table whose rows were never cleared: what stands past the held pages names pages of others."""
+    c = Cache(sequences=3, width=6, pages=10, page_size=4, heads=1, dim=8, layers=2)
+    c.model.table = [[0, 1, 4, 5, 6, 7], [4, 5, 0, 0, 0, 0], [0, 1, 2, 3, 4, 5]]
+    c.model.held, c.model.length = [2, 2, 0], [30, 7, 11]       # lengths past the held pages, too
+    c.model.refcount = [1, 1, 0, 0, 1, 1, 0, 0, 0, 0]
+    c.up()
+    k = c.k.clone()
+    c.compact([[0, 2], [0, 3], [1, 2]], [2, 2, 2])
+    torch.cuda.synchronize()
+    assert c.length.tolist() == [30, 8, 11] and torch.equal(c.k, k)      # (node 0 of the second sequence stays where it is)
+    c.model.length = [30, 8, 11]
+    c.fork([-1, 2, 0])                           # a parent without pages, and one whose length is past its pages
+    torch.cuda.synchronize()
+    assert c.length.tolist() == [30, 0, 8] and c.held.tolist() == [2, 0, 2]
+    assert c.table.tolist()[1:] == [[-1] * 6, [0, 1, -1, -1, -1, -1]]
+    assert c.refcount.tolist() == [2, 2, 0, 0, 0, 0, 0, 0, 0, 0]
+
+
+def test_offsets_past_32_bits():
+    """Pages whose elements lie past 2^31: appended to, attended, compacted and forked."""
+    heads, dim, ps, pages = 8, 128, 64, 36000    # 65536 elements a page: the last ones lie past 2.3e9
+    c = Cache(sequences=2, width=4, pages=4, page_size=ps, heads=heads, dim=dim, layers=1)
+    c.model = Pool(2, 4, pages, ps)
+    c.k, c.v = (torch.empty((1, pages, ps, heads, dim), dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    used = [35999, 7, 35990, 32768]
+    for t in (c.k, c.v):
+        for p in used:
+            t[0, p] = torch.randn((ps, heads, dim), device="cuda")
+    c.model.table = [[35999, 7, 35990, 32768], [-1] * 4]
+    c.model.held, c.model.length = [4, 0], [150, 0]
+    c.model.refcount = [1] * (pages - 1) + [0]
+    c.model.refcount[35999], c.model.refcount[35995] = 1, 0
+    c.up()
+    nodes = 40
+    q = torch.randn((nodes, heads + 2 * heads, dim), device="cuda").to(torch.bfloat16)
+    out, start = torch.empty((nodes, heads, dim), dtype=torch.bfloat16, device="cuda"), i32([0, nodes, nodes])
+    c.append(rope_plan(dim, 0, False), q[:, :heads], out, q[:, heads:2 * heads], q[:, 2 * heads:], start)
+    torch.cuda.synchronize()
+    assert torch.equal(out, q[:, :heads])        # (no pair is turned)
+    for i in range(nodes):
+        p, t = c.model.place(0, 150 + i)
+        assert torch.equal(c.k[0, p, t], q[i, heads:2 * heads]) and torch.equal(c.v[0, p, t], q[i, 2 * heads:])
+    bits = np.tril(np.ones((nodes, nodes), bool))
+    got = torch.empty_like(out)
+    c.attend(out, got, start, words(bits), scale=dim ** -0.5)
+    torch.cuda.synchronize()
+
+    small = Pool(2, 4, 4, ps)                    # the pages that are used, for the 64-bit numbers
+    small.table, small.held, small.length = [[0, 1, 2, 3], [-1] * 4], [4, 0], [150, 0]
+    want, bound = attention(f64(out), small, f64(c.k[0][used]), f64(c.v[0][used]), [0, nodes, nodes], bits, dim ** -0.5, "bf16")
+    assert (np.abs(f64(got) - want) <= bound).all()
+    c.compact([[0, 5, 9], [0, 0, 0]], [3, 0])
+    torch.cuda.synchronize()
+    for i, n in enumerate((0, 5, 9)):
+        p, t = c.model.place(0, 150 + i)
+        assert torch.equal(c.k[0, p, t], q[n, heads:2 * heads])
+    c.model.length = [153, 0]
+    c.fork([-1, 0])                              # the ragged page lands in page 35995
+    torch.cuda.synchronize()
+    assert c.table.tolist()[1] == [35999, 7, 35995, -1]
+    assert torch.equal(c.k[0, 35995, :25], c.k[0, 35990, :25]) and torch.equal(c.v[0, 35995, :25], c.v[0, 35990, :25])

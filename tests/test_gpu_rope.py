@@ -129,7 +129,7 @@ def test_append_where_there_is_no_page():
     """Positions past the held pages, past the table and in a page that is none: the queries are rotated, nothing is written."""
     c = Cache(sequences=4, width=2, pages=4, page_size=4, heads=1, dim=64)
     c.model.table = [[0, -1], [1, 7], [2, 3], [-9, 2**31 - 1]]
-    c.model.length = [3, 3, 7, 2**31 - 1]
+    c.model.length, c.model.held = [3, 3, 7, 2**31 - 1], [2, 2, 2, 2]
     c.up()
     q = torch.randn((8, 2, 64)).to(torch.bfloat16).cuda()
     k = torch.randn((8, 1, 64)).to(torch.bfloat16).cuda()

@@ -50,12 +50,17 @@ int launch_dependent(void (*kernel)(Formal...), dim3 grid, dim3 block, size_t sm
   CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, static_cast<Formal>(args)...));
   return B200Q_OK;
 }
-// Page of position `pos` of sequence `s`, or -1 where the table has none in the pool.
+// Pages that sequence `s` holds, within its row of the table.
+__device__ __forceinline__ int kv_held(const b200q_kv_pool& pool, int s) {
+  const int n = pool.held[s];
+  return n < 0 ? 0 : n < pool.table_width ? n : pool.table_width;
+}
+// Page of position `pos` of sequence `s`, or -1 where it holds none of the pool.
 __device__ __forceinline__ int kv_page(const b200q_kv_pool& pool, int s, int pos) {
   const int j = (int)((unsigned)pos / (unsigned)pool.page_size);
   if (pos < 0 || j >= pool.table_width) return -1;
-  const int p = pool.table[s * pool.table_stride + j];
-  return (unsigned)p < (unsigned)pool.pages ? p : -1;
+  const int p = pool.table[s * pool.table_stride + j];   // (read beside held, not after it)
+  return j < kv_held(pool, s) && (unsigned)p < (unsigned)pool.pages ? p : -1;
 }
 // Element offset of (page, slot of pos) in one layer's keys or values, head 0; -1 where there is no page.
 __device__ __forceinline__ int64_t kv_entry(const b200q_kv_cache& c, const b200q_kv_pool& pool, int s, int pos) {

@@ -197,8 +197,7 @@ __global__ void __launch_bounds__(PLAN_THREADS, 2) reserve_kernel(b200q_kv_pool 
   int held = 0, narrow = 0;
   if (s < pool.sequences && extra[s] >= 0) {
     const int n = pool.length[s];
-    held = pool.held[s];
-    held = held < 0 ? 0 : held < pool.table_width ? held : pool.table_width;
+    held = kv_held(pool, s);
     const long long want = ((long long)(n < 0 ? 0 : n) + extra[s] + pool.page_size - 1) / pool.page_size;
     need = want > held ? want - held : 0;
     narrow = want > pool.table_width;
@@ -231,8 +230,7 @@ __global__ void __launch_bounds__(128) free_kernel(b200q_kv_pool pool, const int
   ptx::griddep_launch_dependents();
   ptx::griddep_wait();
   if (which[s] == 0) return;
-  int n = pool.held[s];
-  n = n < pool.table_width ? n : pool.table_width;
+  const int n = kv_held(pool, s);
   int32_t* row = pool.table + s * pool.table_stride;
   for (int j = threadIdx.x; j < n; j += blockDim.x) {
     const int p = row[j];
@@ -261,7 +259,8 @@ __global__ void __launch_bounds__(PLAN_THREADS, 2) fork_plan_kernel(b200q_kv_poo
   const ForkScratch f = fork_scratch(pool.scratch, n);
   ptx::griddep_launch_dependents();
   ptx::griddep_wait();
-  if (s < n) lengths[s] = kv_length(pool, s);
+  // (positions without pages are not passed on)
+  if (s < n) lengths[s] = (int)min((int64_t)kv_length(pool, s), (int64_t)kv_held(pool, s) * pool.page_size);
   __syncthreads();
   const int p = s < n ? parent[s] : -1;
   const bool child = p >= 0 && p < n && p != s;
@@ -378,7 +377,7 @@ compact_kernel(b200q_kv_cache cache, b200q_kv_pool pool, const int32_t* __restri
   ptx::griddep_launch_dependents();
   ptx::griddep_wait();
   const int blocks_each = (parts + parts_each - 1) / parts_each, s = blockIdx.x / blocks_each, part0 = blockIdx.x % blocks_each * parts_each;
-  const int length = kv_length(pool, s);
+  const int length = pool.length[s];
   int n = path_length[s];
   n = n < 0 ? 0 : n < path_width ? n : path_width;
   if (threadIdx.x == 0) good = n;
@@ -424,10 +423,10 @@ int check_scratch(const char* who, const b200q_kv_pool* pool) {
   return B200Q_OK;
 }
 
-// Raises a kernel's shared-memory limit to what a bitmap of this pool's pages takes.
+// Shared memory of a bitmap of this pool's pages, within the kernel's raised limit.
 int bitmap_bytes(const void* kernel, int pages, size_t* bytes) {
   *bytes = ((size_t)pages + 31) / 32 * 4;
-  if (*bytes > 32 * 1024) CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, KV_MAX_PAGES / 8));
+  CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, KV_MAX_PAGES / 8));
   return B200Q_OK;
 }
 

@@ -200,7 +200,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap km, const __grid_const
     // ---- what is not seen
     const int p0 = at.unit * UNIT;
     const uint64_t in_pool = ring.there[count++ % ring.NOTES];
-    const bool drafted = p0 + UNIT > at.length;
+    const bool drafted = p0 + UNIT > min(at.length, at.total);   // or past the sequence's end: what lies there is anybody's
     uint64_t see[2] = {~0ull, ~0ull};
     bool fix = false;
     if (drafted || in_pool != ~0ull) {

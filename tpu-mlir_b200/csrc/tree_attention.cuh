@@ -39,8 +39,10 @@ struct SplitItem {
 };
 
 struct Sequence {
-  int first_row, nodes, length, total;   // total: committed positions and nodes
+  int first_row, nodes, length, total;   // total: committed positions and nodes, as far as pages are held
 };
+// (rows without a single page still have a unit, in which they see nothing)
+__device__ __forceinline__ int units_of(int total) { return total > 0 ? (int)(((unsigned)total + UNIT - 1) / UNIT) : 1; }
 __device__ __forceinline__ Sequence load_sequence(const AttnArgs& a, int s) {
   Sequence q;
   const int64_t b = a.io.row_start[s], e = a.io.row_start[s + 1];
@@ -48,8 +50,8 @@ __device__ __forceinline__ Sequence load_sequence(const AttnArgs& a, int s) {
   q.first_row = (int)b;
   q.nodes = b >= 0 && end > b ? (int)(end - b) : 0;
   q.length = kv_length(a.pool, s);
-  const int64_t most = (int64_t)a.pool.table_width * a.pool.page_size, all = (int64_t)q.length + q.nodes;
-  q.total = (int)(all < most ? all : most);
+  const int64_t held = (int64_t)kv_held(a.pool, s) * a.pool.page_size, all = (int64_t)q.length + q.nodes;
+  q.total = (int)(all < held ? all : held);
   return q;
 }
 
@@ -129,7 +131,7 @@ struct Place {
     const Sequence q = line.seqs[seq];
     s = seq;
     tiles = (int)(((long long)q.nodes * line.group + line.tile_rows - 1) / line.tile_rows);
-    units = (q.total + UNIT - 1) / UNIT;
+    units = units_of(q.total);
     total = q.total;
     length = q.length;
     nodes = q.nodes;
@@ -182,7 +184,7 @@ __device__ __forceinline__ long long lay_out(const AttnArgs& a, int tile_rows, i
     if (s >= n) break;
     const Sequence q = load_sequence(a, s);
     const long long tiles = ((long long)q.nodes * a.group + tile_rows - 1) / tile_rows;
-    mine += a.cache.heads * tiles * ((q.total + UNIT - 1) / UNIT + cost);
+    mine += a.cache.heads * tiles * (units_of(q.total) + cost);
     seqs[s] = q;
     sums[s] = mine;
   }
@@ -264,7 +266,8 @@ __device__ __forceinline__ void load_units(const AttnArgs& a, const CUtensorMap*
   Slot<STAGES> at_stage(1);     // the first pass over the ring finds it empty
   uint32_t sent = 0;
   // what a lane knows of its unit: the table's entry for its box (as it stands there, so that nothing waits for it; -1: none) and slot of
-  // the box's first row, cache head, rows up to the sequence's end (0: the run is over)
+  // the box's first row, cache head, rows up to the sequence's end (RUN_OVER: no unit)
+  constexpr int RUN_OVER = -0x7fffffff;
   struct Found {
     int page[2], slot[2], head, rows;
   };
@@ -278,7 +281,7 @@ __device__ __forceinline__ void load_units(const AttnArgs& a, const CUtensorMap*
   };
   auto look_up = [&]() {
     Found f;
-    f.rows = at.pos < end ? at.total - at.unit * UNIT : 0;
+    f.rows = at.pos < end ? at.total - at.unit * UNIT : RUN_OVER;
     f.head = at.head;
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
@@ -286,7 +289,7 @@ __device__ __forceinline__ void load_units(const AttnArgs& a, const CUtensorMap*
       f.page[j] = -1;
       f.slot[j] = 0;
       if (b < boxes && b * box < f.rows) {
-        // (total is within the table)
+        // (total is within the pages that are held, and those within the table)
         f.page[j] = a.pool.table[at.s * a.pool.table_stride + (unsigned)pos / (unsigned)page_size];
         f.slot[j] = (int)((unsigned)pos % (unsigned)page_size);
       }
@@ -303,7 +306,7 @@ __device__ __forceinline__ void load_units(const AttnArgs& a, const CUtensorMap*
     for (int g = 0; g < group; ++g) {
       const int first = boxes < 32 ? g * boxes : 0;   // the lane that knows the unit's first box
       const int here = __shfl_sync(0xffffffffu, now.rows, first), head = __shfl_sync(0xffffffffu, now.head, first);
-      if (here == 0) {
+      if (here == RUN_OVER) {
         more = false;
         break;
       }

@@ -380,7 +380,7 @@ tree_attention_umma_kernel(const __grid_constant__ CUtensorMap km, const __grid_
         // ---- what is not seen
         const int p0 = (started + u) * UNIT;
         const uint64_t in_pool = ring.there[unit % ring.NOTES];
-        const bool drafted = p0 + UNIT > at.length;
+        const bool drafted = p0 + UNIT > min(at.length, at.total);   // or past the sequence's end: what lies there is anybody's
         uint64_t see = ~0ull;
         bool fix = false;
         if (drafted || in_pool != ~0ull) {
