@@ -710,7 +710,7 @@ int b200q_rope_append_dev(const b200q_rope_plan *plan, const b200q_kv_cache *cac
  * A row that sees nothing (and one whose scores are all -inf) becomes zeros; what a row does not see does not touch it, infinities
  * and NaN included.  Positions without a page are not seen.  Rows outside every sequence stay as they are.  Products and sums in
  * fp32, the weights rounded to the 16-bit type before the second product.  q, out 16-byte aligned with strides of multiples of 8
- * elements; scale positive.  workspace: b200q_tree_attention_workspace bytes, 16-byte aligned, contents irrelevant before and after;
+ * elements; out may be q (the same strides) and must not overlap it otherwise; scale positive.  workspace: b200q_tree_attention_workspace bytes, 16-byte aligned, contents irrelevant before and after;
  * calls that can overlap (two captured graphs replayed at a time among them) need one each. */
 typedef struct {
   const void *q;

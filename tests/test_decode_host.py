@@ -221,3 +221,25 @@ def test_frequencies(lib, rotary, base, kind, factor, span, low, high):
     assert all(x == 0 for x in p.frequency[rotary // 2:])
     if kind in ("yarn", "banded"):
         assert max(f) <= 1.0 and min(f) >= base ** (-1 + 2 / rotary) / factor * (1 - 1e-12)
+
+
+def test_arrays_of_words_are_aligned(lib):
+    c, p, odd = C.byref(cache()), C.byref(pool()), FAKE + 2
+    for rc in (lib.b200q_kv_reserve_dev(p, odd, None, None), lib.b200q_kv_reserve_dev(p, FAKE, odd, None), lib.b200q_kv_free_dev(p, odd, None),
+               lib.b200q_kv_fork_dev(c, p, odd, None, None), lib.b200q_kv_fork_dev(c, p, FAKE, odd, None),
+               lib.b200q_kv_compact_dev(c, p, odd, 4, 4, FAKE, FAKE + 4096, None), lib.b200q_kv_compact_dev(c, p, FAKE, 4, 4, odd, FAKE + 4096, None),
+               lib.b200q_kv_compact_dev(c, p, FAKE, 4, 4, FAKE, odd, None),
+               lib.b200q_tree_attention_dev(c, p, C.byref(attention(row_start=odd)), None), lib.b200q_tree_attention_dev(c, p, C.byref(attention(status=odd)), None)):
+        refused(lib, rc, L.ERR_INVALID, b"4-byte aligned")
+
+
+def test_limits_of_32_bit_counts(lib):
+    """What would be counted past 32 bits: a tile's rows behind the last one, pieces of a page behind the last one."""
+    for rows in ((1 << 31) - 1, (1 << 31) - 200):
+        refused(lib, lib.b200q_tree_attention_dev(C.byref(cache()), C.byref(pool()), C.byref(attention(rows=rows, q_heads=2)), None), L.ERR_UNSUPPORTED, b"rows")
+    big = cache(heads=65535, head_dim=256)      # 2097120 pieces a slot
+    refused(lib, lib.b200q_kv_fork_dev(C.byref(big), C.byref(pool(page_size=600)), FAKE, None, None), L.ERR_UNSUPPORTED, b"page")
+
+
+def test_attention_in_place_wants_the_same_strides(lib):
+    refused(lib, lib.b200q_tree_attention_dev(C.byref(cache()), C.byref(pool()), C.byref(attention(out_row_stride=512)), None), L.ERR_INVALID, b"in place")

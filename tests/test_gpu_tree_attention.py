@@ -222,3 +222,62 @@ def test_many_sequences():
     rng = np.random.default_rng(1)
     n = 1024
     check(*setup([int(x) for x in rng.integers(0, 3, n)], [int(x) for x in rng.integers(0, 40, n)], heads=1, group=1, dim=16, seed=50))
+
+
+@pytest.mark.parametrize("group,counts,lengths", [(1, [1, 5], [70, 3000]), (4, [6, 2], [2000, 0]), (4, [20, 9], [1500, 64]), (4, [64], [1100])])
+def test_in_place(group, counts, lengths):
+    c, q, start, bits = setup(counts, lengths, group=group, dim=128, seed=60)
+    out = torch.empty_like(q)
+    c.attend(q, out, i32(start), words(bits))
+    c.attend(q, q, i32(start), words(bits))
+    torch.cuda.synchronize()
+    assert torch.equal(q, out)
+
+
+@pytest.mark.parametrize("nodes,dim", [(1, 64), (6, 64), (12, 64), (40, 64), (1, 256)])
+def test_many_small_weights_beside_a_large_one(nodes, dim):
+    """8000 weights of 2^-25.5, each less than half the smallest half precision number, beside one of 1 whose value is 0: together they are
+    the result.  All sequences read the same pages; there are enough of them that most contexts are not cut."""
+    n, length, ps, group = 600, 8000, 16, 4
+    pages = length // ps
+    c = Cache(sequences=n, width=pages + 4, pages=pages, page_size=ps, heads=1, dim=dim, dtype="f16", seed=70)
+    c.model.table = [list(range(pages)) + [-1] * 4 for _ in range(n)]      # the nodes have no pages: only the context is seen
+    c.model.length, c.model.held = [length] * n, [pages] * n
+    c.up()
+    c.k.zero_()
+    c.v.fill_(1.0)
+    c.k[0, 0, 0, 0, 0] = 4.0
+    c.v[0, 0, 0].zero_()
+    q = torch.zeros((n * nodes, group, dim), dtype=torch.float16, device="cuda")
+    q[:, :, 0] = 25.5 * np.log(2) / 4
+    out = torch.full_like(q, 9.0)
+    c.attend(q, out, torch.arange(0, (n + 1) * nodes, nodes, dtype=torch.int32, device="cuda"), None, scale=1.0)
+    torch.cuda.synchronize()
+    w = np.exp(-4.0 * float(q[0, 0, 0]))
+    want = (length - 1) * w / (1 + (length - 1) * w)
+    # weights are multiples of 2^-24 / 2^7: half of that each; the score in fp32 (|score| 2^-22); the sum's 2^-23 a term; the result's rounding
+    bound = (length - 1) * 2.0**-32 + want * (17.7 * 2.0**-22 + length * 2.0**-23 + 2.0**-11)
+    assert float((out.double() - want).abs().max()) <= bound, (float(out.min()), float(out.max()), want, bound)
+
+
+@pytest.mark.parametrize("group", [1, 40])
+def test_positions_up_to_the_last_of_31_bits(group):
+    """A context whose last unit starts at 2^31 - 64 (of two pages: one of them stands in the table over and over).  With queries of zero
+    all weights are 1 and the sums are whole numbers below 2^24 in every block."""
+    ps, width = 16, 2**27 - 1
+    c = Cache(sequences=1, width=1, pages=2, page_size=ps, heads=1, dim=64, seed=80)
+    c.model.length, c.model.held = [width * ps - 3], [width]
+    c.up()
+    c.table = torch.zeros((1, width), dtype=torch.int32, device="cuda")
+    c.table[0, -1] = 1
+    c.v.zero_()
+    c.v[0, 0, :, 0, 0] = 1.0
+    c.v[0, 0, 0, 0, 1] = 8.0
+    c.v[0, 1, -1, 0, :] = float("nan")        # the last node: only itself sees it
+    q = torch.zeros((3, group, 64), dtype=torch.bfloat16, device="cuda")
+    out = torch.full_like(q, 9.0)
+    c.attend(q, out, i32([0, 3]), None, scale=1.0)
+    torch.cuda.synchronize()
+    assert bool(out[2].isnan().all())
+    # 16 of 2^31 positions have other values than those below: nothing beside half a step of bf16
+    assert bool((out[:2, :, 0] == 1.0).all()) and bool((out[:2, :, 1] == 0.5).all()) and bool((out[:2, :, 2:] == 0).all())

@@ -3,6 +3,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <initializer_list>
+
 #include "internal.h"
 
 namespace b200q {
@@ -13,6 +15,8 @@ constexpr int KV_MAX_HEAD_DIM = 256;
 
 int kv_check_pool(const char* who, const b200q_kv_pool* pool);
 int kv_check_cache(const char* who, const b200q_kv_cache* cache);
+// 32-bit arguments whose addresses the device takes as they are (null: not given)
+int kv_check_words(const char* who, std::initializer_list<const void*> words);
 
 // Makes the device that holds `p` current for the life of the object (the launch goes to that device whichever one the
 // caller has current); rc is not B200Q_OK when `p` is no device memory.

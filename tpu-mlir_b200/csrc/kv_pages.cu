@@ -43,6 +43,12 @@ int kv_check_cache(const char* who, const b200q_kv_cache* cache) {
   return B200Q_OK;
 }
 
+int kv_check_words(const char* who, std::initializer_list<const void*> words) {
+  for (const void* p : words)
+    if ((uintptr_t)p & 3) return set_error(B200Q_ERR_INVALID, "%s: an array of 32-bit numbers is not 4-byte aligned", who);
+  return B200Q_OK;
+}
+
 OnDeviceOf::OnDeviceOf(const char* who, const void* p) {
   cudaPointerAttributes a{};
   cudaError_t e = cudaPointerGetAttributes(&a, p);
@@ -232,7 +238,7 @@ __global__ void __launch_bounds__(128) free_kernel(b200q_kv_pool pool, const int
   if (which[s] == 0) return;
   const int n = kv_held(pool, s);
   int32_t* row = pool.table + s * pool.table_stride;
-  for (int j = threadIdx.x; j < n; j += blockDim.x) {
+  for (unsigned j = threadIdx.x; j < (unsigned)n; j += blockDim.x) {   // (n may be 2^31 - 1)
     const int p = row[j];
     if ((unsigned)p < (unsigned)pool.pages) atomicSub(pool.refcount + p, 1);
     row[j] = -1;
@@ -310,14 +316,17 @@ fork_kernel(b200q_kv_cache cache, b200q_kv_pool pool, const int32_t* __restrict_
   ptx::griddep_wait();
   if (*f.go == 0) return;
   if ((int)blockIdx.x < table_blocks) {
-    for (int c0 = blockIdx.x * columns; c0 < pool.table_width; c0 += table_blocks * columns) {
+    // (64 bits: a row of the table may have 2^31 - 1 entries)
+    for (int64_t c0 = (int64_t)blockIdx.x * columns; c0 < pool.table_width; c0 += table_blocks * columns) {
       for (int i = threadIdx.x; i < n * columns; i += FORK_THREADS) {
-        const int s = i / columns, c = c0 + i % columns;
+        const int s = i / columns;
+        const int64_t c = c0 + i % columns;
         old[i] = c < pool.table_width ? pool.table[s * pool.table_stride + c] : -1;
       }
       __syncthreads();
       for (int i = threadIdx.x; i < n * columns; i += FORK_THREADS) {
-        const int s = i / columns, c = c0 + i % columns, p = parent[s];
+        const int s = i / columns, p = parent[s];
+        const int64_t c = c0 + i % columns;
         if (p < 0 || p >= n || p == s || c >= pool.table_width) continue;
         const int full = f.length[p] / pool.page_size;
         int entry = -1;
@@ -442,6 +451,7 @@ int64_t b200q_kv_scratch_words(int32_t sequences) { return scratch_words(sequenc
 int b200q_kv_reserve_dev(const b200q_kv_pool* pool, const int32_t* extra, int32_t* status, void* stream) {
   B200Q_TRY(kv_check_pool("kv_reserve", pool));
   if (!extra) return set_error(B200Q_ERR_INVALID, "kv_reserve: null extra");
+  B200Q_TRY(kv_check_words("kv_reserve", {extra, status}));
   if (pool->sequences == 0) return B200Q_OK;
   OnDeviceOf dev("kv_reserve", pool->table);
   B200Q_TRY(dev.rc);
@@ -453,6 +463,7 @@ int b200q_kv_reserve_dev(const b200q_kv_pool* pool, const int32_t* extra, int32_
 int b200q_kv_free_dev(const b200q_kv_pool* pool, const int32_t* which, void* stream) {
   B200Q_TRY(kv_check_pool("kv_free", pool));
   if (!which) return set_error(B200Q_ERR_INVALID, "kv_free: null which");
+  B200Q_TRY(kv_check_words("kv_free", {which}));
   if (pool->sequences == 0) return B200Q_OK;
   OnDeviceOf dev("kv_free", pool->table);
   B200Q_TRY(dev.rc);
@@ -464,8 +475,9 @@ int b200q_kv_fork_dev(const b200q_kv_cache* cache, const b200q_kv_pool* pool, co
   B200Q_TRY(kv_check_cache("kv_fork", cache));
   B200Q_TRY(check_scratch("kv_fork", pool));
   if (!parent) return set_error(B200Q_ERR_INVALID, "kv_fork: null parent");
-  if ((int64_t)pool->page_size * cache->heads * (cache->head_dim / 8) > 0x7fffffffLL)
-    return set_error(B200Q_ERR_UNSUPPORTED, "kv_fork: a page of one layer has more than 2^31 - 1 pieces of 16 bytes");
+  B200Q_TRY(kv_check_words("kv_fork", {parent, status}));
+  if ((int64_t)pool->page_size * cache->heads * (cache->head_dim / 8) > 1 << 30)
+    return set_error(B200Q_ERR_UNSUPPORTED, "kv_fork: a page of one layer has more than 2^30 pieces of 16 bytes");
   if (pool->sequences == 0) return B200Q_OK;
   OnDeviceOf dev("kv_fork", pool->table);
   B200Q_TRY(dev.rc);
@@ -478,7 +490,8 @@ int b200q_kv_fork_dev(const b200q_kv_cache* cache, const b200q_kv_pool* pool, co
   // 32 columns a tile where they fit, at least 2
   int columns = FORK_TILE / pool->sequences;
   columns = columns > 32 ? 32 : columns;
-  const int tiles = ceil_div(pool->table_width, columns), table_blocks = tiles < sms ? tiles : sms;
+  const int64_t tiles = ((int64_t)pool->table_width + columns - 1) / columns;
+  const int table_blocks = (int)(tiles < sms ? tiles : sms);
   const int64_t copies = (int64_t)pool->sequences * 2 * cache->layers;
   const int copy_blocks = (int)(copies < FORK_PER_SM * sms ? copies : FORK_PER_SM * sms);
   return launch_dependent(fork_kernel, dim3(table_blocks + copy_blocks), dim3(FORK_THREADS), 0, s, *cache, *pool, parent, table_blocks, columns);
@@ -489,6 +502,7 @@ int b200q_kv_compact_dev(const b200q_kv_cache* cache, const b200q_kv_pool* pool,
   B200Q_TRY(kv_check_pool("kv_compact", pool));
   B200Q_TRY(kv_check_cache("kv_compact", cache));
   if (!path || !path_length || !length_out) return set_error(B200Q_ERR_INVALID, "kv_compact: null argument");
+  B200Q_TRY(kv_check_words("kv_compact", {path, path_length, length_out}));
   if (path_width < 0 || path_stride < path_width) return set_error(B200Q_ERR_INVALID, "kv_compact: bad shape of the paths");
   if (path_width > PATH_MOST) return set_error(B200Q_ERR_UNSUPPORTED, "kv_compact: a path has at most %d nodes", PATH_MOST);
   const bool in_place = length_out == pool->length;

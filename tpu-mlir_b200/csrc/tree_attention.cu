@@ -200,7 +200,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap km, const __grid_const
     // ---- what is not seen
     const int p0 = at.unit * UNIT;
     const uint64_t in_pool = ring.there[count++ % ring.NOTES];
-    const bool drafted = p0 + UNIT > min(at.length, at.total);   // or past the sequence's end: what lies there is anybody's
+    const bool drafted = p0 > min(at.length, at.total) - UNIT;   // or past the sequence's end: what lies there is anybody's
     uint64_t see[2] = {~0ull, ~0ull};
     bool fix = false;
     if (drafted || in_pool != ~0ull) {
@@ -245,7 +245,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap km, const __grid_const
       for (int t = 0; t < NT; ++t) top = fmaxf(top, fmaxf(sc[t][2 * h], sc[t][2 * h + 1]));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      const float now = fmaxf(m[h], top * a.scale_log2), base = now == -INFINITY ? 0.f : now;
+      const float now = fmaxf(m[h], top * a.scale_log2), base = now == -INFINITY ? 0.f : now, lifted = base - lift<F16>();
       alpha[h] = exp2_approx(m[h] - base);
       m[h] = now;
       float sum = 0.f;
@@ -253,7 +253,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap km, const __grid_const
       for (int t = 0; t < NT; ++t)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const float p = exp2_approx(fmaf(sc[t][2 * h + e], a.scale_log2, -base));
+          const float p = exp2_approx(fmaf(sc[t][2 * h + e], a.scale_log2, -lifted));
           sc[t][2 * h + e] = p;
           sum += p;
         }
@@ -521,7 +521,16 @@ int launch(const AttnArgs& a, int sms, cudaStream_t s) {
   return launch_join(a, blocks, S::ROWS, DIM, s);
 }
 
-// Rows of a tile by the batch's average of (node, head of the group) a cache head, which the host knows.
+// Rows of a tile by the batch's average of (node, head of the group) a cache head, which the host knows.  Both sides of each rule, bf16:
+//   up to 16 rows, 16-row tiles on mma.sync: 4 rows x 48 sequences of 200..8000 at dim 128 81.5 us (tcgen05 tiles 107.2), 4 rows x one of
+//     430 12.6 (32-row tiles 15.3, tcgen05 14.7), 16 rows x 16 sequences of 700..5000 41.7 (47.1), 8 rows x 64 of 20..600 29.4 (43.1);
+//   up to 32 rows, 32-row tiles: 24 x 16 sequences 43.1 (47.1), 32 x 16 45.0 (48.3), 32 x 64 short ones 37.7 (44.2), 20 rows x one of
+//     131,000 at dim 64 44.4 (45.0); from 48 rows on a 64-row tile of the same kernel was slower than tcgen05 (49 x 120,000, dim 64:
+//     55.2 against 43.2), and at dim 128 it spilled (96 rows x 16 sequences: 163 against 47), so there is none;
+//   more rows: tcgen05, 128 rows a tile, two streams of units a block.  Above 128 rows the two streams take two row tiles and share each
+//     unit's keys and values: 160 rows x 8 sequences of 700..8000 49.9 (two streams of one tile: 63.5), 512 rows 91.2 (124.5); below, one
+//     tile would idle: 96 rows 40.4 shared out by units against 44.5.
+// Heads of more than 128 keep the 32-row tile: their scores and sums of two streams do not fit tensor memory beside one another.
 template <bool F16, int DIM>
 int launch_rows(const AttnArgs& a, int sms, cudaStream_t s) {
   const int64_t rows = (a.io.rows + a.pool.sequences - 1) / a.pool.sequences * a.group;
@@ -586,15 +595,17 @@ int b200q_tree_attention_dev(const b200q_kv_cache* cache, const b200q_kv_pool* p
   if (!io.q || !io.out || !io.row_start || !io.workspace) return set_error(B200Q_ERR_INVALID, "tree_attention: null argument");
   if (io.rows < 0 || io.rows > 0x7fffffffLL || io.q_heads < 1 || io.q_heads % cache->heads)
     return set_error(B200Q_ERR_INVALID, "tree_attention: rows must fit 31 bits and q_heads be a multiple of the cache's heads");
-  if (io.rows * (io.q_heads / cache->heads) > 0x7fffffffLL) return set_error(B200Q_ERR_UNSUPPORTED, "tree_attention: too many rows");
+  // (a tile's rows are counted in 32 bits, past the last row too)
+  if (io.rows * (io.q_heads / cache->heads) > 0x7fffffffLL - 2 * UMMA_ROWS) return set_error(B200Q_ERR_UNSUPPORTED, "tree_attention: too many rows");
   if (io.layer < 0 || io.layer >= cache->layers) return set_error(B200Q_ERR_INVALID, "tree_attention: no layer %d in the cache", io.layer);
   if (!(io.scale > 0.f) || !isfinite(io.scale)) return set_error(B200Q_ERR_INVALID, "tree_attention: scale must be positive");
   if (((uintptr_t)io.q | (uintptr_t)io.out | (uintptr_t)io.workspace) & 15)
     return set_error(B200Q_ERR_INVALID, "tree_attention: q, out and workspace must be 16-byte aligned");
-  if (((uintptr_t)io.row_start | (uintptr_t)io.mask) & 3)
-    return set_error(B200Q_ERR_INVALID, "tree_attention: row_start and mask must be 4-byte aligned");
+  B200Q_TRY(kv_check_words("tree_attention", {io.row_start, io.mask, io.status}));
   if ((io.q_row_stride | io.q_head_stride | io.out_row_stride | io.out_head_stride) & 7)
     return set_error(B200Q_ERR_INVALID, "tree_attention: strides of q and out must be multiples of 8 elements");
+  if (io.q == io.out && (io.q_row_stride != io.out_row_stride || io.q_head_stride != io.out_head_stride))
+    return set_error(B200Q_ERR_INVALID, "tree_attention: in place, the strides of q and out must be the same");
   if (io.mask && io.mask_stride < 0) return set_error(B200Q_ERR_INVALID, "tree_attention: negative mask_stride");
   if (io.rows == 0 || pool->sequences == 0) return B200Q_OK;
   OnDeviceOf dev("tree_attention", pool->table);

@@ -86,6 +86,13 @@ __device__ __forceinline__ uint32_t pack_pair(float lo, float hi) {
   const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
+// Weights are 2^lift times what the formula says (sums alike, so the quotient is the formula's): the smallest half precision number is
+// 2^-24, and a long context's many weights below half of that beside one large weight would all be rounded to nothing.  They are at most
+// 1, or 2^8 where sums are rescaled late, so 2^7 stays below 65504.  bfloat16 reaches 2^-133.
+template <bool F16>
+__device__ __forceinline__ constexpr float lift() {
+  return F16 ? 7.f : 0.f;
+}
 // a 16-bit number that is infinite or NaN
 template <bool F16>
 __device__ __forceinline__ bool not_finite(uint32_t bits) {

@@ -380,7 +380,7 @@ tree_attention_umma_kernel(const __grid_constant__ CUtensorMap km, const __grid_
         // ---- what is not seen
         const int p0 = (started + u) * UNIT;
         const uint64_t in_pool = ring.there[unit % ring.NOTES];
-        const bool drafted = p0 + UNIT > min(at.length, at.total);   // or past the sequence's end: what lies there is anybody's
+        const bool drafted = p0 > min(at.length, at.total) - UNIT;   // or past the sequence's end: what lies there is anybody's
         uint64_t see = ~0ull;
         bool fix = false;
         if (drafted || in_pool != ~0ull) {
@@ -446,7 +446,7 @@ tree_attention_umma_kernel(const __grid_constant__ CUtensorMap km, const __grid_
         const uint32_t turn = PAIR ? 2 * unit + stream : unit;
         if (turn) rows_sync<COMPUTERS>(4 + (turn & 1));
         // ---- weights (rounded to the 16-bit type: what the tensor cores take; the rounding is unbiased and averages out over positions)
-        const float base = m == -INFINITY ? 0.f : m;
+        const float base = (m == -INFINITY ? 0.f : m) - lift<F16>();
         uint32_t p[2][16];   // two weights a word
         const float2 scale2 = make_float2(a.scale_log2, a.scale_log2), base2 = make_float2(-base, -base);
         float2 sum2 = make_float2(0.f, 0.f);
