@@ -48,9 +48,8 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// What an item costs, in units (48 sequences of one token: 91 / 84.5 / 81.6 / 81.6 us at 1 / 2 / 3 / 4), and the shortest run of units that is
-// worth a block (one token at 430 positions: 13 us at one unit, 14 at two, 16 at four, 20 at eight).
-constexpr int ITEM_COST = 3, MIN_UNITS = 1;
+// What an item costs, in units (48 sequences of one token: 91 / 84.5 / 81.6 / 81.6 us at 1 / 2 / 3 / 4).
+constexpr int ITEM_COST = 3;
 constexpr int COMPUTERS = 128, BLOCK = COMPUTERS + 32 * LOADERS;
 
 __device__ __forceinline__ void computers_sync() { asm volatile("barrier.cta.sync 1, 128;" ::: "memory"); }
@@ -112,8 +111,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap km, const __grid_const
   const long long total = lay_out<BLOCK>(a, S::ROWS, ITEM_COST, seqs, sums, scan_buf);
   const Line line{seqs, a.pool.sequences, a.cache.heads, group, S::ROWS, ITEM_COST};
 
-  long long run = (total + gridDim.x - 1) / gridDim.x;
-  if (run < MIN_UNITS + ITEM_COST) run = MIN_UNITS + ITEM_COST;
+  const long long run = run_of(total);
   const long long u0 = (long long)blockIdx.x * run, u1 = u0 + run < total ? u0 + run : total;
   if (tid == 0) a.items[blockIdx.x].parts = 0;
   if (u0 >= u1) return;
@@ -200,7 +198,8 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap km, const __grid_const
     // ---- what is not seen
     const int p0 = at.unit * UNIT;
     const uint64_t in_pool = ring.there[count++ % ring.NOTES];
-    const bool drafted = p0 > min(at.length, at.total) - UNIT;   // or past the sequence's end: what lies there is anybody's
+    const int first_drafted = min(at.length, at.total);
+    const bool drafted = p0 > first_drafted - UNIT;   // or past the sequence's end: what lies there is anybody's
     uint64_t see[2] = {~0ull, ~0ull};
     bool fix = false;
     if (drafted || in_pool != ~0ull) {
@@ -217,21 +216,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap km, const __grid_const
       if (drafted) {
         // Values of drafted nodes meet weights of zero in rows that do not see them: infinite or NaN ones are taken out of the
         // tile (and added below where they are seen), or they would make those rows NaN.
-        bool found = false;
-        for (int c = tid; c < UNIT * PIECES; c += COMPUTERS) {
-          const int row = c / PIECES;
-          uint32_t* w = reinterpret_cast<uint32_t*>(smem + (vs - smem_base) + tile_at(row, c % PIECES));
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const uint32_t x = w[j];
-            const bool lo = not_finite<F16>(x & 0xffffu), hi = not_finite<F16>(x >> 16);
-            if (lo || hi) {
-              found = true;
-              w[j] = (lo ? 0u : x & 0xffffu) | (hi ? 0u : x & 0xffff0000u);
-              atomicOr(&bad[row >> 5], 1u << (row & 31));
-            }
-          }
-        }
+        const bool found = clean_values<F16, PIECES>(smem + (vs - smem_base), first_drafted > p0 ? first_drafted - p0 : 0, tid, COMPUTERS, bad);
         fix = computers_or(found);
       }
     }

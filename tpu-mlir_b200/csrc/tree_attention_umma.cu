@@ -26,8 +26,8 @@ namespace {
 constexpr int ROWS = UMMA_ROWS, COMPUTERS = 2 * ROWS, MAKERS = COMPUTERS / 32 + LOADERS;   // two streams of rows, loading warps,
 constexpr int BLOCK = 32 * (MAKERS + 2);                                                      // a warp a stream that issues products
 // What an item costs, in units (16 trees of 24 nodes 52.1 / 50.4 / 49.0 / 48.1 us at 2 / 4 / 6 / 8, 50.5 at 16; queries, the first scores, the
-// sums' way out), and the shortest run of units that is worth a block.
-constexpr int ITEM_COST = 8, MIN_UNITS = 1;
+// sums' way out).
+constexpr int ITEM_COST = 8;
 constexpr float SLACK = 8.f;                         // log2 of how far weights may exceed 1
 
 // B operand that is contiguous along N: blocks of 64 elements (128-byte swizzle) `lead` bytes apart, groups of 8 rows of K 1024 apart
@@ -241,8 +241,7 @@ tree_attention_umma_kernel(const __grid_constant__ CUtensorMap km, const __grid_
   ptx::tc_fence_before_sync();
   const long long total = lay_out<BLOCK>(a, TILE_ROWS, ITEM_COST, seqs, sums, scan_buf);
   const Line line{seqs, a.pool.sequences, a.cache.heads, group, TILE_ROWS, ITEM_COST};
-  long long run = (total + gridDim.x - 1) / gridDim.x;
-  if (run < MIN_UNITS + ITEM_COST) run = MIN_UNITS + ITEM_COST;
+  const long long run = run_of(total);
   const long long u0 = (long long)blockIdx.x * run, u1 = u0 + run < total ? u0 + run : total;
   if (tid == 0) a.items[blockIdx.x].parts = 0;
   ptx::tc_fence_after_sync();   // (lay_out ends with the block's barrier)
@@ -380,7 +379,8 @@ tree_attention_umma_kernel(const __grid_constant__ CUtensorMap km, const __grid_
         // ---- what is not seen
         const int p0 = (started + u) * UNIT;
         const uint64_t in_pool = ring.there[unit % ring.NOTES];
-        const bool drafted = p0 > min(at.length, at.total) - UNIT;   // or past the sequence's end: what lies there is anybody's
+        const int first_drafted = min(at.length, at.total);
+        const bool drafted = p0 > first_drafted - UNIT;   // or past the sequence's end: what lies there is anybody's
         uint64_t see = ~0ull;
         bool fix = false;
         if (drafted || in_pool != ~0ull) {
@@ -391,21 +391,8 @@ tree_attention_umma_kernel(const __grid_constant__ CUtensorMap km, const __grid_
           if (drafted) {
             // infinite and NaN values of drafted nodes leave the tile: rows that do not see them would become NaN (tree_attention.cu)
             wait(&ring.full[unit % RING], unit / RING & 1, 9);
-            bool found = false;
-            for (int c = PAIR ? tid : row_in; c < UNIT * PIECES; c += SHARERS) {
-              const int row = c / PIECES;
-              uint32_t* w = reinterpret_cast<uint32_t*>(smem + (stages - q_tile) + (unit % RING * 2 + 1) * S::TILE + tile_at(row, c % PIECES));
-#pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                const uint32_t x = w[j];
-                const bool lo = not_finite<F16>(x & 0xffffu), hi = not_finite<F16>(x >> 16);
-                if (lo || hi) {
-                  found = true;
-                  w[j] = (lo ? 0u : x & 0xffffu) | (hi ? 0u : x & 0xffff0000u);
-                  atomicOr(&bad_rows[row >> 5], 1u << (row & 31));
-                }
-              }
-            }
+            const bool found = clean_values<F16, PIECES>(smem + (stages - q_tile) + (unit % RING * 2 + 1) * S::TILE, first_drafted > p0 ? first_drafted - p0 : 0,
+                                                         PAIR ? tid : row_in, SHARERS, bad_rows);
             if (found) ptx::fence_proxy_async_smem();
             fix = rows_or<SHARERS>(bar_rows, found);
           }
