@@ -152,12 +152,12 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap km, const __grid_const
       for (int h = 0; h < 2; ++h) {
         const int r = at.tile * S::ROWS + wr * 16 + lane / 4 + 8 * h;
         const bool real = r < at.nodes * group;
-        const int t = r / group, row = at.first_row + (real ? t : 0);
+        const int t = (unsigned)r / (unsigned)group, row = at.first_row + (real ? t : 0);
         node[h] = t;
         if (a.io.mask && a.io.mask_stride && (lane & 3) == 0) prefetch(a.io.mask + (int64_t)row * a.io.mask_stride);
         m[h] = -INFINITY;
         l[h] = 0.f;
-        const uint16_t* src = static_cast<const uint16_t*>(a.io.q) + (int64_t)row * a.io.q_row_stride + (at.head * group + r % group) * a.io.q_head_stride;
+        const uint16_t* src = static_cast<const uint16_t*>(a.io.q) + (int64_t)row * a.io.q_row_stride + (at.head * group + r - t * group) * a.io.q_head_stride;
 #pragma unroll
         for (int k = 0; k < DIM / 16; ++k) {
           const int d = k * 16 + (lane & 3) * 2;
@@ -381,8 +381,8 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap km, const __grid_const
           if (r >= at.nodes * group) continue;
           if (whole) {
             const float inv = l[h] == 0.f ? 0.f : 1.f / l[h];
-            uint16_t* dst = static_cast<uint16_t*>(a.io.out) + (int64_t)(at.first_row + r / group) * a.io.out_row_stride +
-                            (at.head * group + r % group) * a.io.out_head_stride;
+            uint16_t* dst = static_cast<uint16_t*>(a.io.out) + (int64_t)(at.first_row + node[h]) * a.io.out_row_stride +
+                            (at.head * group + r - node[h] * group) * a.io.out_head_stride;
 #pragma unroll
             for (int k = 0; k < DIM / 8; ++k) {
               const int d = k * 8 + (lane & 3) * 2;

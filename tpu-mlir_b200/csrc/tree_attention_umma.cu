@@ -323,6 +323,9 @@ tree_attention_umma_kernel(const __grid_constant__ CUtensorMap km, const __grid_
     uint32_t* const bad_rows = bad[PAIR ? 0 : stream];
     const uint16_t* vp = static_cast<const uint16_t*>(a.cache.v) + a.io.layer * a.cache.layer_stride;
     const uint32_t mine = tmem + ((uint32_t)(warp & 3) << 21) + stream * S::STREAM;   // this warp's 32 lanes of its stream's columns
+    constexpr int STEP = (PAIR ? ROWS : COMPUTERS) / PIECES;   // rows between a thread's pieces of the queries
+    const int step_t = STEP / group, step_h = STEP - step_t * group;
+    const int64_t step_from = step_t * a.io.q_row_stride + step_h * a.io.q_head_stride, carry_from = a.io.q_row_stride - group * a.io.q_head_stride;
     uint32_t done = 0;    // steps of this stream so far
     uint32_t unit = 0;    // units of the run so far
     while (at.pos < u1) {
@@ -333,16 +336,28 @@ tree_attention_umma_kernel(const __grid_constant__ CUtensorMap km, const __grid_
       const int r0 = at.tile * TILE_ROWS + (PAIR ? stream * ROWS : 0), rows = at.nodes * group;
       {
         // 16 bytes a thread and copy, all of them in flight together (loaded and stored one after the other they took 6000 clocks and more)
-        constexpr int LOADING = PAIR ? ROWS : COMPUTERS, STEP = LOADING / PIECES;
         const int at0 = PAIR ? row_in : tid, piece = at0 % PIECES, row0 = at0 / PIECES;
         const uint32_t dst = q_tile + (PAIR ? stream * S::QUERIES : 0) + (piece >> 3) * (ROWS * 128);
         const uint16_t* src = static_cast<const uint16_t*>(a.io.q) + (int64_t)at.first_row * a.io.q_row_stride + (int64_t)at.head * group * a.io.q_head_stride;
+        // One division for (node, head of the group), then STEP rows further each: a division a row took as long as the loads.  Addresses go on
+        // by sums or by products, whichever the rest of the loop came out better with (PAIR: 512 rows x 8 sequences 81.3 and 88.0 us; not
+        // PAIR: 96 rows 41.3 and 38.4).
+        int t = (unsigned)(r0 + row0) / (unsigned)group, h = r0 + row0 - t * group;
+        int64_t from = (int64_t)t * a.io.q_row_stride + h * a.io.q_head_stride;
 #pragma unroll
         for (int i = 0; i < ROWS / STEP; ++i) {
-          const int row = row0 + i * STEP, r = r0 + row, t = r / group;
-          const bool in = r < rows && piece * 8 < dim;
+          const int row = row0 + i * STEP;
+          const bool in = r0 + row < rows && piece * 8 < dim;
           cp_async16(dst + row * 128 + (((piece & 7) ^ (row & 7)) * 16),
-                     in ? src + (int64_t)t * a.io.q_row_stride + (r - t * group) * a.io.q_head_stride + piece * 8 : src, in);
+                     in ? src + (PAIR ? from : (int64_t)t * a.io.q_row_stride + h * a.io.q_head_stride) + piece * 8 : src, in);
+          h += step_h;
+          t += step_t;
+          from += step_from;
+          if (h >= group) {
+            h -= group;
+            ++t;
+            from += carry_from;
+          }
         }
         cp_async_wait_all();
       }
@@ -354,7 +369,7 @@ tree_attention_umma_kernel(const __grid_constant__ CUtensorMap km, const __grid_
         for (int j = 0; j < 2; ++j)
           if (units > 1 || (unit & 1) == j) ptx::mbar_arrive(ptx::smem_u32(&q_full[j]));
       }
-      const int r = r0 + row_in, node = r / group;
+      const int r = r0 + row_in, node = (unsigned)r / (unsigned)group;
       const bool real = r < rows;
       if (a.io.mask && a.io.mask_stride && real) prefetch(a.io.mask + (int64_t)(at.first_row + node) * a.io.mask_stride);
       float m = -INFINITY, l = 0.f;
@@ -510,7 +525,7 @@ tree_attention_umma_kernel(const __grid_constant__ CUtensorMap km, const __grid_
       const bool had0 = !fresh, had1 = !PAIR && (units > 1 || fresh);   // this stream, the other: had a unit at all
       const float inv = l == 0.f ? 0.f : 1.f / l;
       uint16_t* dst = static_cast<uint16_t*>(a.io.out) + (int64_t)(at.first_row + (real ? node : 0)) * a.io.out_row_stride +
-                      (at.head * group + r % group) * a.io.out_head_stride;
+                      (at.head * group + r - node * group) * a.io.out_head_stride;
       float* part = a.partial + (blockIdx.x * 2 + (started == 0)) * part_size(TILE_ROWS, DIM);
       const int part_row = (PAIR ? stream * ROWS : 0) + row_in;
       const uint32_t theirs = mine ^ S::STREAM;   // (the allocation starts at a multiple of its size)
