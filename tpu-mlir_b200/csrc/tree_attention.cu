@@ -13,7 +13,7 @@
 // Two warps of a block only load, one keys and one values, with TMA boxes of as many rows as both a page and a unit are made of, ahead of
 // the products and across items, into a ring of stages of 64 keys and values; four warps compute.  Shared memory holds 64 elements
 // a row, swizzled by 16-byte pieces (piece ^ row % 8), so that ldmatrix meets no bank twice.  (Loading with 16-byte cp.async took 640
-// instructions a warp and unit: 108 us for 48 sequences of one token, 450 MB, that take 81.5 this way: 5.5 TB/s, 0.84 of the measured rate.)
+// instructions a warp and unit: 108 us for 48 sequences of one token, 450 MB, that take 80 this way: 5.6 TB/s, 0.86 of the measured rate.)
 //
 // What bounds it: DRAM; 10 us of a launch, the batch's lengths, the first unit's way through table and memory, and the join are fixed.
 #include <math.h>
