@@ -281,3 +281,30 @@ def test_positions_up_to_the_last_of_31_bits(group):
     assert bool(out[2].isnan().all())
     # 16 of 2^31 positions have other values than those below: nothing beside half a step of bf16
     assert bool((out[:2, :, 0] == 1.0).all()) and bool((out[:2, :, 1] == 0.5).all()) and bool((out[:2, :, 2:] == 0).all())
+
+
+@pytest.mark.parametrize("dim,group,counts,lengths", [(64, 4, [700, 3, 129], [0, 500, 70]), (128, 1, [300, 513], [0, 63]), (64, 7, [200, 90], [130, 0]),
+                                                      (256, 2, [150], [40]), (64, 1, [1], [0]), (16, 3, [17, 40, 11], [65, 0, 64]), (128, 40, [30], [100])])
+def test_long_chains(dim, group, counts, lengths):
+    """Chains of many row tiles, each of which ends at its own last node."""
+    check(*setup(counts, lengths, dim=dim, group=group, heads=2, tree=False, before=1, after=2, seed=dim + group), scale=dim ** -0.5)
+
+
+def test_long_chain_without_all_of_its_pages():
+    c, q, start, _ = setup([400], [100], dim=64, group=4, tree=False, seed=90)
+    c.model.held[0] = 20                            # 320 positions: later nodes see no more than these
+    c.model.table[0][9] = -1
+    c.up()
+    check(c, q, start, None)
+
+
+def test_what_is_not_seen_in_a_long_chain():
+    """Infinities and NaN that only later nodes of a chain see, in the same unit and in later ones."""
+    c, q, start, _ = setup([300], [50], dim=64, group=4, tree=False, seed=91)
+    plain = check(c, q, start, None)
+    for node, bad in ((40, float("nan")), (130, float("inf")), (131, -float("inf"))):
+        p, slot = c.model.place(0, 50 + node)
+        c.v[0, p, slot, :, 5] = bad
+        c.k[0, p, slot, :, 7] = bad if node == 40 else 1.0
+    out = check(c, q, start, None)
+    assert torch.equal(out[:40], plain[:40]) and not bool(torch.isfinite(out[40:]).all())

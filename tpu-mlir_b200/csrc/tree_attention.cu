@@ -108,14 +108,14 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap km, const __grid_const
     ptx::prefetch_tensormap(&vm);
   }
   ptx::griddep_wait();
-  const long long total = lay_out<BLOCK>(a, S::ROWS, ITEM_COST, seqs, sums, scan_buf);
-  const Line line{seqs, a.pool.sequences, a.cache.heads, group, S::ROWS, ITEM_COST};
+  const long long total = lay_out<BLOCK, false>(a, S::ROWS, ITEM_COST, seqs, sums, scan_buf);
+  const Line<false> line{seqs, a.pool.sequences, a.cache.heads, group, S::ROWS, ITEM_COST};
 
   const long long run = run_of(total);
   const long long u0 = (long long)blockIdx.x * run, u1 = u0 + run < total ? u0 + run : total;
   if (tid == 0) a.items[blockIdx.x].parts = 0;
   if (u0 >= u1) return;
-  Place at;
+  Place<false> at;
   at.find(line, sums, u0);
   const uint16_t* vp = static_cast<const uint16_t*>(a.cache.v) + a.io.layer * a.cache.layer_stride;
   const uint32_t smem_base = ptx::smem_u32(smem);
@@ -198,8 +198,8 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap km, const __grid_const
     // ---- what is not seen
     const int p0 = at.unit * UNIT;
     const uint64_t in_pool = ring.there[count++ % ring.NOTES];
-    const int first_drafted = min(at.length, at.total);
-    const bool drafted = p0 > first_drafted - UNIT;   // or past the sequence's end: what lies there is anybody's
+    const int unseen = min(at.length, at.total);
+    const bool drafted = p0 > unseen - UNIT;   // or past the sequence's end: what lies there is anybody's
     uint64_t see[2] = {~0ull, ~0ull};
     bool fix = false;
     if (drafted || in_pool != ~0ull) {
@@ -216,7 +216,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap km, const __grid_const
       if (drafted) {
         // Values of drafted nodes meet weights of zero in rows that do not see them: infinite or NaN ones are taken out of the
         // tile (and added below where they are seen), or they would make those rows NaN.
-        const bool found = clean_values<F16, PIECES>(smem + (vs - smem_base), first_drafted > p0 ? first_drafted - p0 : 0, tid, COMPUTERS, bad);
+        const bool found = clean_values<F16, PIECES>(smem + (vs - smem_base), unseen > p0 ? unseen - p0 : 0, tid, COMPUTERS, bad);
         fix = computers_or(found);
       }
     }
@@ -515,13 +515,15 @@ int launch(const AttnArgs& a, int sms, cudaStream_t s) {
 //   more rows: tcgen05, 128 rows a tile, two streams of units a block.  Above 128 rows the two streams take two row tiles and share each
 //     unit's keys and values: 160 rows x 8 sequences of 700..8000 49.9 (two streams of one tile: 63.5), 512 rows 91.2 (124.5); below, one
 //     tile would idle: 96 rows 40.4 shared out by units against 44.5.
+// Chains of more than two row tiles on average (prompts) take the form in which tiles end at their own last node (a prompt of 4096 nodes
+// 158 us, without 491; in short calls its formula costs 1 us of 10).
 // Heads of more than 128 keep the 32-row tile: their scores and sums of two streams do not fit tensor memory beside one another.
 template <bool F16, int DIM>
 int launch_rows(const AttnArgs& a, int sms, cudaStream_t s) {
   const int64_t rows = (a.io.rows + a.pool.sequences - 1) / a.pool.sequences * a.group;
   if (rows <= 16) return launch<F16, DIM, 1, 4>(a, sms, s);
   if (rows <= 32 || DIM > 128) return launch<F16, DIM, 2, 2>(a, sms, s);
-  return launch_umma(a, rows > UMMA_ROWS, sms, s);
+  return launch_umma(a, rows > UMMA_ROWS, !a.io.mask && rows > 2 * UMMA_ROWS, sms, s);
 }
 
 template <bool F16>

@@ -192,7 +192,7 @@ struct Shape {
   static size_t bytes(int sequences) { return 1024 + FIXED + (size_t)sequences * (sizeof(long long) + sizeof(Sequence)); }
 };
 
-template <bool F16, int DIM, bool PAIR>
+template <bool F16, int DIM, bool PAIR, bool GROWS>
 __global__ void __launch_bounds__(BLOCK, 1)
 tree_attention_umma_kernel(const __grid_constant__ CUtensorMap km, const __grid_constant__ CUtensorMap vm, const __grid_constant__ AttnArgs a) {
   using S = Shape<DIM, PAIR>;
@@ -241,8 +241,8 @@ tree_attention_umma_kernel(const __grid_constant__ CUtensorMap km, const __grid_
     ptx::tmem_relinquish();
   }
   ptx::tc_fence_before_sync();
-  const long long total = lay_out<BLOCK>(a, TILE_ROWS, ITEM_COST, seqs, sums, scan_buf);
-  const Line line{seqs, a.pool.sequences, a.cache.heads, group, TILE_ROWS, ITEM_COST};
+  const long long total = lay_out<BLOCK, GROWS>(a, TILE_ROWS, ITEM_COST, seqs, sums, scan_buf);
+  const Line<GROWS> line{seqs, a.pool.sequences, a.cache.heads, group, TILE_ROWS, ITEM_COST};
   const long long run = run_of(total);
   const long long u0 = (long long)blockIdx.x * run, u1 = u0 + run < total ? u0 + run : total;
   if (tid == 0) a.items[blockIdx.x].parts = 0;
@@ -254,7 +254,7 @@ tree_attention_umma_kernel(const __grid_constant__ CUtensorMap km, const __grid_
     return;
   }
 
-  Place at;
+  Place<GROWS> at;
   at.find(line, sums, u0);
   // A wait that runs out ends all waiting: the roles go on without (or stop, where they would load or multiply), and the status says
   // so.
@@ -396,8 +396,8 @@ tree_attention_umma_kernel(const __grid_constant__ CUtensorMap km, const __grid_
         // ---- what is not seen
         const int p0 = (started + u) * UNIT;
         const uint64_t in_pool = ring.there[unit % ring.NOTES];
-        const int first_drafted = min(at.length, at.total);
-        const bool drafted = p0 > first_drafted - UNIT;   // or past the sequence's end: what lies there is anybody's
+        const int unseen = at.unseen(line);
+        const bool drafted = p0 > unseen - UNIT;   // or past the sequence's end: what lies there is anybody's
         uint64_t see = ~0ull;
         bool fix = false;
         if (drafted || in_pool != ~0ull) {
@@ -408,7 +408,7 @@ tree_attention_umma_kernel(const __grid_constant__ CUtensorMap km, const __grid_
           if (drafted) {
             // infinite and NaN values of drafted nodes leave the tile: rows that do not see them would become NaN (tree_attention.cu)
             wait(&ring.full[unit % RING], unit / RING & 1, 9);
-            const bool found = clean_values<F16, PIECES>(smem + (stages - q_tile) + (unit % RING * 2 + 1) * S::TILE, first_drafted > p0 ? first_drafted - p0 : 0,
+            const bool found = clean_values<F16, PIECES>(smem + (stages - q_tile) + (unit % RING * 2 + 1) * S::TILE, unseen > p0 ? unseen - p0 : 0,
                                                          PAIR ? tid : row_in, SHARERS, bad_rows);
             if (found) ptx::fence_proxy_async_smem();
             fix = rows_or<SHARERS>(bar_rows, found);
@@ -575,10 +575,10 @@ tree_attention_umma_kernel(const __grid_constant__ CUtensorMap km, const __grid_
   if (warp == MAKERS) ptx::tmem_dealloc(tmem, S::COLUMNS);
 }
 
-template <bool F16, int DIM, bool PAIR>
+template <bool F16, int DIM, bool PAIR, bool GROWS>
 int launch(const AttnArgs& a, int sms, cudaStream_t s) {
   using S = Shape<DIM, PAIR>;
-  auto kernel = tree_attention_umma_kernel<F16, DIM, PAIR>;
+  auto kernel = tree_attention_umma_kernel<F16, DIM, PAIR, GROWS>;
   CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::bytes(KV_MAX_SEQUENCES)));
   CUtensorMap km, vm;
   B200Q_TRY(make_map(&km, a, a.cache.k));
@@ -586,17 +586,21 @@ int launch(const AttnArgs& a, int sms, cudaStream_t s) {
   B200Q_TRY(launch_dependent(kernel, dim3(sms), dim3(BLOCK), S::bytes(a.pool.sequences), s, km, vm, a));
   return launch_join(a, sms, S::TILES * ROWS, DIM, s);
 }
+template <bool F16, int DIM>
+int launch_form(const AttnArgs& a, bool pair, bool grows, int sms, cudaStream_t s) {
+  if (grows) return launch<F16, DIM, true, true>(a, sms, s);
+  return pair ? launch<F16, DIM, true, false>(a, sms, s) : launch<F16, DIM, false, false>(a, sms, s);
+}
 template <bool F16>
-int launch_dim(const AttnArgs& a, bool pair, int sms, cudaStream_t s) {
-  if (a.cache.head_dim <= 64) return pair ? launch<F16, 64, true>(a, sms, s) : launch<F16, 64, false>(a, sms, s);
-  return pair ? launch<F16, 128, true>(a, sms, s) : launch<F16, 128, false>(a, sms, s);
+int launch_dim(const AttnArgs& a, bool pair, bool grows, int sms, cudaStream_t s) {
+  return a.cache.head_dim <= 64 ? launch_form<F16, 64>(a, pair, grows, sms, s) : launch_form<F16, 128>(a, pair, grows, sms, s);
 }
 
 }  // namespace
 
 namespace attn {
-int launch_umma(const AttnArgs& a, bool pair, int sms, cudaStream_t s) {
-  return a.cache.dtype == B200Q_DT_F16 ? launch_dim<true>(a, pair, sms, s) : launch_dim<false>(a, pair, sms, s);
+int launch_umma(const AttnArgs& a, bool pair, bool grows, int sms, cudaStream_t s) {
+  return a.cache.dtype == B200Q_DT_F16 ? launch_dim<true>(a, pair, grows, sms, s) : launch_dim<false>(a, pair, grows, sms, s);
 }
 }  // namespace attn
 }  // namespace b200q
