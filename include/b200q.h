@@ -620,8 +620,8 @@ typedef struct {
 
 /* Which pages a sequence holds.  Position p of sequence s lies in page table[s * table_stride + p / page_size], slot
  * p % page_size, for p / page_size < held[s] <= table_width; it has no page past that, or where the table's entry is none of the
- * pool's.  Entries past held[s] are not read (-1 where a call here cleared them).  length[s] positions are committed; refcount[p] sequences hold page p, 0 means free.  A new pool is refcount = 0,
- * held = 0, length = 0.  `scratch` is working space of at least b200q_kv_scratch_words(sequences) words whose contents need not be
+ * pool's.  Entries past held[s] count for nothing (-1 where a call here cleared them).  length[s] positions are committed;
+ * refcount[p] sequences hold page p, 0 means free.  A new pool is refcount = 0, held = 0, length = 0.  `scratch` is working space of at least b200q_kv_scratch_words(sequences) words whose contents need not be
  * kept: calls that use it (fork, compact) and can overlap need pools with scratch of their own.  Limits: 1024 sequences,
  * 1048576 pages, table_width * page_size below 2^31. */
 typedef struct {
@@ -642,8 +642,8 @@ int b200q_kv_free_dev(const b200q_kv_pool *pool, const int32_t *which, void *str
 /* Every sequence s with a parent[s] other than s in [0, sequences) becomes what that sequence was BEFORE the call (beams
  * reordered in one call; swaps and several children of one parent included); other values of parent leave s alone.  Full
  * pages are shared; the filled slots of a ragged last page are copied in every layer into a page of the child's own (the
- * lowest-numbered pages free before the call, in the order of the sequences); pages held past the parent's length are not passed on, nor positions without a page;
- * what s held is given back after that.  When the free pages do not suffice nothing changes and *status (optional) becomes 1. */
+ * lowest-numbered pages free before the call, in the order of the sequences); pages held past the parent's length are not
+ * passed on, nor positions without a page; what s held is given back after that.  When the free pages do not suffice nothing changes and *status (optional) becomes 1. */
 int b200q_kv_fork_dev(const b200q_kv_cache *cache, const b200q_kv_pool *pool, const int32_t *parent, int32_t *status, void *stream);
 /* Keeps the accepted path of a tree of drafted tokens whose entries stand at positions length[s] + node: for i below
  * path_length[s], in order, the entry of node path[s * path_stride + i] moves to position length[s] + i in every layer, and
@@ -709,7 +709,8 @@ int b200q_rope_append_dev(const b200q_rope_plan *plan, const b200q_kv_cache *cac
  *   out = sum_j w_j v_j / sum_j w_j,  w_j = exp(scale * (q . k_j) - max)
  * A row that sees nothing (and one whose scores are all -inf) becomes zeros; what a row does not see does not touch it, infinities
  * and NaN included.  Positions without a page are not seen.  Rows outside every sequence stay as they are.  Products and sums in
- * fp32, the weights rounded to the 16-bit type before the second product.  q, out 16-byte aligned with strides of multiples of 8
+ * fp32, the weights rounded to the 16-bit type before the second product (half precision ones times 2^7, which the sums take out
+ * again: small ones stay).  q, out 16-byte aligned with strides of multiples of 8
  * elements; out may be q (the same strides) and must not overlap it otherwise; scale positive.  workspace: b200q_tree_attention_workspace bytes, 16-byte aligned, contents irrelevant before and after;
  * calls that can overlap (two captured graphs replayed at a time among them) need one each. */
 typedef struct {

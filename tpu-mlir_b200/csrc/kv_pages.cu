@@ -123,7 +123,8 @@ __device__ __noinline__ uint32_t free_one_by_one(const int32_t* refcount, int at
 }
 
 // The `need` lowest free pages, in order: give(first, rank, page, mine) is called by whole warps, `mine` once for every rank below `need`;
-// `first` is the rank of the warp's first free page.  Nothing is called and false returned when there are fewer.  All threads of a block of PLAN_THREADS call it; bitmap: a word for 32 pages.
+// `first` is the rank of the warp's first free page.  Nothing is called and false returned when there are fewer.  All threads of a block of
+// PLAN_THREADS call it; bitmap: a word for 32 pages.
 //
 // Free pages become bits (a lane looks at four counts, eight lanes' nibbles make a word), 16384 pages a step so that all loads of a
 // step are in flight, and the steps end once enough are found.  Then, 1024 words a step, ranks are the sums of the bits before (a scan),
