@@ -216,7 +216,9 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap km, const __grid_const
       if (drafted) {
         // Values of drafted nodes meet weights of zero in rows that do not see them: infinite or NaN ones are taken out of the
         // tile (and added below where they are seen), or they would make those rows NaN.
+        // The stage's next values come by TMA, which does not wait for ordinary stores by itself: the fence puts these before them.
         const bool found = clean_values<F16, PIECES>(smem + (vs - smem_base), unseen > p0 ? unseen - p0 : 0, tid, COMPUTERS, bad);
+        if (found) ptx::fence_proxy_async_smem();
         fix = computers_or(found);
       }
     }
