@@ -643,7 +643,7 @@ int b200q_kv_free_dev(const b200q_kv_pool *pool, const int32_t *which, void *str
  * reordered in one call; swaps and several children of one parent included); other values of parent leave s alone.  Full
  * pages are shared; the filled slots of a ragged last page are copied in every layer into a page of the child's own (the
  * lowest-numbered pages free before the call, in the order of the sequences); pages held past the parent's length are not
- * passed on, nor positions without a page; what s held is given back after that.  When the free pages do not suffice nothing changes and *status (optional) becomes 1. */
+ * passed on, nor positions without a page (no free page is taken for them); what s held is given back after that.  When the free pages do not suffice nothing changes and *status (optional) becomes 1. */
 int b200q_kv_fork_dev(const b200q_kv_cache *cache, const b200q_kv_pool *pool, const int32_t *parent, int32_t *status, void *stream);
 /* Keeps the accepted path of a tree of drafted tokens whose entries stand at positions length[s] + node: for i below
  * path_length[s], in order, the entry of node path[s * path_stride + i] moves to position length[s] + i in every layer, and

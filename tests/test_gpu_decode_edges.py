@@ -44,3 +44,41 @@ def test_stages_that_are_filled_again_after_infinities_were_taken_out(nodes, gro
     rows = np.concatenate([np.arange(s * nodes, (s + 1) * nodes) for s in some])
     want, bound = attention(f64(q[rows]), c.model, f64(c.k[0]), f64(c.v[0]), list(range(0, len(rows) + 1, nodes)), bits[rows], dim ** -0.5, dtype)
     assert (np.abs(f64(out[rows]) - want) <= bound).all()
+
+
+@pytest.mark.parametrize("bad", [-1, 40, 2**31 - 1, -2**31])
+def test_fork_of_a_ragged_page_that_is_none(bad):
+    """The child has no page where its parent has none: no free page is taken for it, and attention sees the same positions of both."""
+    c = Cache(sequences=4, width=4, pages=12, page_size=16, heads=2, dim=64, layers=2, seed=3)
+    c.model.table = [[3, 5, bad, -1], [7, -1, -1, -1], [9, bad, 4, 8], [1, -1, -1, -1]]
+    c.model.length, c.model.held = [40, 9, 45, 16], [3, 1, 4, 1]
+    c.model.refcount = [0, 1, 0, 1, 1, 1, 0, 1, 1, 1, 0, 0]
+    c.up()
+    k, v = c.k.clone(), c.v.clone()
+    c.fork([-1, 0, -1, 2])
+    torch.cuda.synchronize()
+    # the second sequence has no page at column 2, the fourth a hole at column 1 and a copy of page 4 (13 slots) in page 0
+    assert c.status.item() == 0
+    assert c.length.tolist() == [40, 40, 45, 45] and c.held.tolist() == [3, 3, 4, 3]
+    assert c.table.tolist() == [[3, 5, bad, -1], [3, 5, -1, -1], [9, bad, 4, 8], [9, bad, 0, -1]]
+    assert c.refcount.tolist() == [1, 0, 0, 2, 1, 2, 0, 0, 1, 2, 0, 0]
+    k[:, 0, :13], v[:, 0, :13] = k[:, 4, :13], v[:, 4, :13]
+    assert torch.equal(c.k, k) and torch.equal(c.v, v)
+    q = torch.randn((1, 4, 64), device="cuda").to(torch.bfloat16).repeat(4, 1, 1)
+    out = torch.empty_like(q)
+    c.attend(q, out, i32([0, 1, 2, 3, 4]))           # (a chain of one node whose position has no page)
+    torch.cuda.synchronize()
+    assert torch.equal(out[0], out[1])
+    c.free([1, 1, 1, 1])
+    torch.cuda.synchronize()
+    assert c.refcount.tolist() == [0] * 12
+
+
+def test_fork_of_a_missing_page_needs_no_free_one():
+    c = Cache(sequences=2, width=2, pages=2, page_size=4, heads=1, dim=8)
+    c.model.table, c.model.length, c.model.held, c.model.refcount = [[0, -1], [1, -1]], [6, 3], [2, 1], [1, 1]
+    c.up()
+    c.fork([-1, 0])
+    torch.cuda.synchronize()
+    assert c.status.item() == 0
+    assert c.table.tolist() == [[0, -1], [0, -1]] and c.length.tolist() == [6, 6] and c.held.tolist() == [2, 2] and c.refcount.tolist() == [2, 0]

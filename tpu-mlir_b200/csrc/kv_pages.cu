@@ -271,7 +271,8 @@ __global__ void __launch_bounds__(PLAN_THREADS, 2) fork_plan_kernel(b200q_kv_poo
   __syncthreads();
   const int p = s < n ? parent[s] : -1;
   const bool child = p >= 0 && p < n && p != s;
-  const int count = child ? lengths[p] : 0, ragged = count % pool.page_size != 0;
+  // a ragged last page that is none of the pool's is passed on as it is: positions without a page
+  const int count = child ? lengths[p] : 0, source = count % pool.page_size ? kv_page(pool, p, count) : -1, ragged = source >= 0;
   int total;
   const int rank = block_scan(ragged, buf, &total) - ragged;
   if (ragged) list[rank] = s;
@@ -279,7 +280,7 @@ __global__ void __launch_bounds__(PLAN_THREADS, 2) fork_plan_kernel(b200q_kv_poo
     f.length[s] = lengths[s];
     f.held[s] = pool.held[s];
     f.page[s] = -1;
-    f.source[s] = ragged ? kv_page(pool, p, count) : -1;
+    f.source[s] = source;
   }
   if (s == 0) {
     *f.ragged = total;
@@ -350,7 +351,6 @@ fork_kernel(b200q_kv_cache cache, b200q_kv_pool pool, const int32_t* __restrict_
   const bool slots_outside = cache.slot_stride >= cache.head_stride;
   for (int item = blockIdx.x - table_blocks; item < ragged * parts; item += gridDim.x - table_blocks) {
     const int s = f.list[item / parts], part = item % parts, from = f.source[s], to = f.page[s];
-    if (from < 0) continue;
     const int slots = f.length[parent[s]] % pool.page_size;
     uint16_t* base = static_cast<uint16_t*>(part & 1 ? cache.v : cache.k) + (part >> 1) * cache.layer_stride;
     const int inner = slots_outside ? cache.heads : slots, count = slots * cache.heads * chunks;
