@@ -6,8 +6,8 @@ import pytest
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
 
-from decode_model import TORCH, attention  # noqa: E402
-from decode_util import Cache, f64, i32, random_tree, words  # noqa: E402
+from decode_model import TORCH, attention, frequencies, rotate, smallest, step  # noqa: E402
+from decode_util import Cache, f64, i32, random_tree, rope_plan, words  # noqa: E402
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f16"])
@@ -82,3 +82,30 @@ def test_fork_of_a_missing_page_needs_no_free_one():
     torch.cuda.synchronize()
     assert c.status.item() == 0
     assert c.table.tolist() == [[0, -1], [0, -1]] and c.length.tolist() == [6, 6] and c.held.tolist() == [2, 2] and c.refcount.tolist() == [2, 0]
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_rows_past_the_table_are_turned_by_where_they_belong(interleaved):
+    """Lengths past what a row of the table holds: nothing is written, the queries are turned by length + node all the same.
+
+    Bound of tests/test_gpu_rope.py; an angle of 2^31 turns carries two 64-bit roundings of 2^-53 * 2^31 each, 2^-21 together."""
+    c = Cache(sequences=5, width=2, pages=10, page_size=4, heads=1, dim=64)
+    c.model.table = [[0, 1], [2, 3], [4, 5], [6, 7], [8, 9]]
+    c.model.length, c.model.held = [8, 1000, 2**31 - 1, 2**31 - 2, -7], [2] * 5
+    c.up()
+    q = torch.randn((10, 2, 64), generator=torch.Generator().manual_seed(1)).to(torch.bfloat16).cuda()
+    k = torch.randn((10, 1, 64), generator=torch.Generator().manual_seed(2)).to(torch.bfloat16).cuda()
+    out, want_v, old_k = torch.zeros_like(q), c.v.clone(), c.k.clone()
+    c.append(rope_plan(64, 64, interleaved), q, out, k, k, i32([0, 2, 4, 6, 8, 10]))
+    torch.cuda.synchronize()
+    at = [8, 9, 1000, 1001, 2**31 - 1, 2**31, 2**31 - 2, 2**31 - 1, 0, 1]       # (a length below zero is an empty sequence)
+    f, m = frequencies(64, 10000.0)
+    want, size = rotate(f64(q), at, f, m, interleaved)
+    size *= np.where(np.array(at) > 2**24, 4.0, 1.0)[:, None, None]
+    bound = step("bf16") * np.abs(want) + (1 + step("bf16")) * 2.0**-21 * size + smallest("bf16")
+    assert (np.abs(f64(out) - want) <= bound).all()
+    want_v[0, 8, 0], want_v[0, 8, 1] = k[8], k[9]
+    assert torch.equal(c.v, want_v)
+    untouched = torch.ones(c.k.shape[:3], dtype=torch.bool, device="cuda")
+    untouched[0, 8, :2] = False
+    assert torch.equal(c.k[untouched], old_k[untouched])

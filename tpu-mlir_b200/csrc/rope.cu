@@ -56,7 +56,8 @@ __host__ __device__ __forceinline__ int turn_size(int half) { return (half + 3) 
 template <bool F16, bool INTERLEAVED, bool WIDE>
 __global__ void __launch_bounds__(ROPE_THREADS) rope_kernel(const __grid_constant__ RopeArgs a) {
   extern __shared__ __align__(16) float2 turn[];   // [rows_per_block][turn_size] (cos, sin), the magnitude in both
-  __shared__ int row_seq[ROPE_ROWS], row_pos[ROPE_ROWS];
+  __shared__ int row_seq[ROPE_ROWS];
+  __shared__ double row_pos[ROPE_ROWS];   // (past 31 bits where a length is near them)
   __shared__ int64_t row_entry[ROPE_ROWS];
   const b200q_rope_append& io = a.io;
   const int half = a.plan.rotary_dim / 2, dim = a.plan.head_dim;
@@ -68,17 +69,18 @@ __global__ void __launch_bounds__(ROPE_THREADS) rope_kernel(const __grid_constan
 
   if (warp < rows) {
     const int64_t r = r0 + warp;
-    int seq = 0, pos = 0;
-    int64_t entry = -1;
+    int seq = 0;
+    int64_t pos = 0, entry = -1;
     if (io.row_start) {
       // the last sequence that starts at or before the row (the starts ascend)
       int before = 0;
       for (int s = lane; s < a.pool.sequences; s += 32) before += io.row_start[s] <= r;
       seq = __reduce_add_sync(0xffffffffu, before) - 1;
       if (seq >= 0 && r < io.row_start[seq + 1]) {
-        const int64_t p = (int64_t)kv_length(a.pool, seq) + (r - io.row_start[seq]);
-        pos = (int)(p < 0x7fffffff ? p : 0x7fffffff);
-        if (p < 0x7fffffff) entry = kv_entry(a.cache, a.pool, seq, pos);
+        // (the length as it is: one past the table's row has no page, but it is where the row belongs)
+        const int length = a.pool.length[seq];
+        pos = (length < 0 ? 0 : length) + (r - io.row_start[seq]);
+        if (pos <= 0x7fffffff) entry = kv_entry(a.cache, a.pool, seq, (int)pos);
       } else {
         seq = -1;
       }
@@ -86,7 +88,7 @@ __global__ void __launch_bounds__(ROPE_THREADS) rope_kernel(const __grid_constan
     if (io.positions) pos = io.positions[r];
     if (lane == 0) {
       row_seq[warp] = seq;
-      row_pos[warp] = pos;
+      row_pos[warp] = (double)pos;
       row_entry[warp] = entry;
     }
   }
@@ -96,7 +98,7 @@ __global__ void __launch_bounds__(ROPE_THREADS) rope_kernel(const __grid_constan
     const int at_once = ROPE_THREADS / half, pair = threadIdx.x % half;
     const double turns_per_position = a.plan.frequency[pair] * 0.15915494309189533577;
     for (int row = threadIdx.x / half; row < rows && (int)threadIdx.x < at_once * half; row += at_once) {
-      double t = (double)row_pos[row] * turns_per_position;
+      double t = row_pos[row] * turns_per_position;
       t -= rint(t);
       float s, c;
       sincospif(2.f * (float)t, &s, &c);
