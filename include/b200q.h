@@ -707,8 +707,8 @@ int b200q_rope_append_dev(const b200q_rope_plan *plan, const b200q_kv_cache *cac
  * that its mask names: bit m % 32 of mask[r * mask_stride + m / 32], words past mask_stride counting as 0.  mask NULL: a
  * chain, m <= n (one row a sequence: plain decoding).
  *   out = sum_j w_j v_j / sum_j w_j,  w_j = exp(scale * (q . k_j) - max)
- * A row that sees nothing (and one whose scores are all -inf) becomes zeros; what a row does not see does not touch it, infinities
- * and NaN included.  Positions without a page are not seen.  Rows outside every sequence stay as they are.  Products and sums in
+ * A row that sees nothing becomes zeros, and so does one whose scores, times scale * log2(e) in fp32, are all -inf; one of them at +inf makes
+ * its row NaN.  What a row does not see does not touch it, infinities and NaN included.  Positions without a page are not seen.  Rows outside every sequence stay as they are.  Products and sums in
  * fp32, the weights rounded to the 16-bit type before the second product (half precision ones times 2^7, which the sums take out
  * again: small ones stay).  q, out 16-byte aligned with strides of multiples of 8
  * elements; out may be q (the same strides) and must not overlap it otherwise; scale positive.  workspace: b200q_tree_attention_workspace bytes, 16-byte aligned, contents irrelevant before and after;

@@ -109,3 +109,37 @@ def test_rows_past_the_table_are_turned_by_where_they_belong(interleaved):
     untouched = torch.ones(c.k.shape[:3], dtype=torch.bool, device="cuda")
     untouched[0, 8, :2] = False
     assert torch.equal(c.k[untouched], old_k[untouched])
+
+
+@pytest.mark.parametrize("tree", [True, False])
+@pytest.mark.parametrize("nodes,group,sequences", [(1, 4, 1), (1, 4, 400), (6, 4, 3), (40, 1, 3), (40, 1, 300), (64, 4, 3), (64, 4, 200), (150, 4, 200)])
+def test_scores_past_fp32_make_their_rows_nan(nodes, group, sequences, tree):
+    """Finite scores whose product with scale * log2(e) is not: no weights can be formed, and zeros would say that nothing was seen.  Items that
+    are cut and whole ones, every form; rows of other heads and sequences are as without them."""
+    lengths = [70] * sequences
+    c = Cache(sequences=sequences, width=16, pages=16 * sequences, page_size=16, heads=2, dim=64, seed=11)
+    assert c.model.reserve([x + nodes for x in lengths]) == 0
+    c.model.length = lengths
+    c.up()
+    q = torch.randn((sequences * nodes, 2 * group, 64), generator=torch.Generator().manual_seed(4)).to(torch.bfloat16).cuda()
+    start, space = i32(list(range(0, (sequences + 1) * nodes, nodes))), c.workspace(2 * group)
+    mask = words(np.concatenate([random_tree(np.random.default_rng(s), nodes) for s in range(sequences)])) if tree else None
+    plain, out = torch.empty_like(q), torch.empty_like(q)
+    c.attend(q, plain, start, mask, scale=1.0, space=space)
+    wild = q.clone()
+    wild[0, 1] = 0
+    wild[0, 1, 3] = 2.0**62                       # 2^62 * 2^64 * 3 * log2(e) is past 2^128, the products alone are not
+    p, slot = c.model.place(0, 5)
+    c.k[0, p, slot, 0, 3] = 2.0**64
+    wild[1:, :group, 3] = 0                       # (what the other rows of this cache head see there does not change)
+    wild[0, [h for h in range(group) if h != 1], 3] = 0
+    quiet = wild.clone()
+    quiet[0, 1] = 0
+    c.attend(quiet, plain, start, mask, scale=3.0, space=space)
+    c.attend(wild, out, start, mask, scale=3.0, space=space)
+    torch.cuda.synchronize()
+    assert bool(torch.isfinite(plain).all())
+    assert bool(out[0, 1].isnan().all())
+    same = torch.ones(out.shape[:2], dtype=torch.bool, device="cuda")
+    same[0, 1] = False
+    assert torch.equal(out[same], plain[same])

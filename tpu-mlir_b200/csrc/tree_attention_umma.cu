@@ -525,7 +525,8 @@ tree_attention_umma_kernel(const __grid_constant__ CUtensorMap km, const __grid_
         m = top;
       }
       const bool had0 = !fresh, had1 = !PAIR && (units > 1 || fresh);   // this stream, the other: had a unit at all
-      const float inv = l == 0.f ? 0.f : 1.f / l;
+      // (a finite score that scale * log2(e) took past fp32 leaves a maximum of infinity and no weights: not a row that sees nothing)
+      const float inv = m == INFINITY ? NAN : l == 0.f ? 0.f : 1.f / l;
       uint16_t* dst = static_cast<uint16_t*>(a.io.out) + (int64_t)(at.first_row + (real ? node : 0)) * a.io.out_row_stride +
                       (at.head * group + r - node * group) * a.io.out_head_stride;
       float* part = a.partial + (blockIdx.x * 2 + (started == 0)) * part_size(TILE_ROWS, DIM);
