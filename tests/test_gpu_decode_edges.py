@@ -8,6 +8,7 @@ pytestmark = pytest.mark.gpu
 
 from decode_model import TORCH, attention, frequencies, rotate, smallest, step  # noqa: E402
 from decode_util import Cache, f64, i32, random_tree, rope_plan, words  # noqa: E402
+from test_gpu_tree_attention import setup  # noqa: E402
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f16"])
@@ -143,3 +144,98 @@ def test_scores_past_fp32_make_their_rows_nan(nodes, group, sequences, tree):
     same = torch.ones(out.shape[:2], dtype=torch.bool, device="cuda")
     same[0, 1] = False
     assert torch.equal(out[same], plain[same])
+
+
+def guarded(q):
+    """An output for q's rows inside a wider buffer of nines, and that buffer."""
+    back = torch.full((q.shape[0] + 8, q.shape[1] + 2, q.shape[2] + 8), 9.0, dtype=q.dtype, device="cuda")
+    return back[4:-4, 1:-1, :q.shape[2]], back
+
+
+def only(back, out, named):
+    """Nothing but the named rows of the output was written."""
+    rest = back.clone()
+    view = rest[4:-4, 1:-1, :out.shape[2]]
+    view[named] = 9.0
+    return bool((rest == 9).all())
+
+
+@pytest.mark.parametrize("group,tree", [(2, True), (2, False), (8, True), (12, True), (50, True), (100, False)])
+@pytest.mark.parametrize("wrong,same_as", [([0, 100, -3, 9], [0, 9, 9, 9]), ([5, 2, 9, 4], [2, 2, 9, 9]), ([-4, 3, 7, 9], [3, 3, 7, 9]),
+                                           ([2**31 - 1, -2**31, 9, 9], [9, 9, 9, 9])])
+def test_row_starts_that_do_not_ascend(wrong, same_as, group, tree):
+    """A sequence whose start is negative or not below its end has no rows, ends are cut to the rows there are; no other row is written, nor a byte
+    behind the workspace."""
+    c, q, start, bits = setup([3, 4, 2], [10, 40, 80], group=group, seed=5, tree=tree)
+    out, back = guarded(q)
+    space = c.attend(q, out, i32(wrong), None if bits is None else words(bits))
+    torch.cuda.synchronize()
+    assert bool((space[-64:] == 0xA5).all())
+    want, bound = attention(f64(q), c.model, f64(c.k[0]), f64(c.v[0]), same_as, bits, 0.125, c.dtype)
+    named = ~np.isnan(want).any((1, 2))
+    assert named.sum() == same_as[-1] - same_as[0]
+    assert only(back, out, torch.from_numpy(named).cuda())
+    assert (np.abs(f64(out)[named] - want[named]) <= bound[named]).all()
+
+
+@pytest.mark.parametrize("group,tree", [(2, True), (2, False), (8, True), (12, True), (50, True), (100, False)])
+def test_lengths_past_the_table(group, tree):
+    """The positions of the held pages are seen, no drafted node is: none has a page."""
+    c, q, start, bits = setup([4, 2], [70, 40], page_size=16, group=group, seed=8, tree=tree)
+    c.model.length = [10**6, 2**31 - 1]
+    c.up()
+    out, back = guarded(q)
+    space = c.attend(q, out, i32(start), None if bits is None else words(bits))
+    torch.cuda.synchronize()
+    assert bool((space[-64:] == 0xA5).all()) and only(back, out, slice(None))
+    c.model.length = [c.model.width * 16] * 2
+    want, bound = attention(f64(q), c.model, f64(c.k[0]), f64(c.v[0]), start, bits, 0.125, c.dtype)
+    assert (np.abs(f64(out) - want) <= bound).all()
+
+
+def test_keys_are_written_only_where_their_rows_have_a_page():
+    """Rows past the held pages, past the table and in pages that are none; keys are turned, values are copied, everything else stays."""
+    c = Cache(sequences=4, width=2, pages=4, page_size=4, heads=2, dim=64, layers=2)
+    c.model.table = [[0, -1], [1, 7], [2, 3], [-9, 2**31 - 1]]
+    c.model.length, c.model.held = [3, 3, 7, 2], [2, 2, 2, 2]
+    c.up()
+    g = torch.Generator().manual_seed(6)
+    q, k, v = (torch.randn((8, h, 64), generator=g).to(torch.bfloat16).cuda() for h in (4, 2, 2))
+    out, want_k, want_v = torch.zeros_like(q), c.k.clone(), c.v.clone()
+    at = [1, 5, 2, 9, 0, 3, 7, 8]
+    c.append(rope_plan(64, 64, True), q, out, k, v, i32([0, 2, 4, 6, 8]), i32(at), layer=1)
+    torch.cuda.synchronize()
+    f, m = frequencies(64, 10000.0)
+    for got, x in ((out, q), (torch.stack([c.k[1, 0, 3], c.k[1, 1, 3], c.k[1, 3, 3]]), k[[0, 2, 4]])):
+        want, size = rotate(f64(x), at if x is q else [at[0], at[2], at[4]], f, m, True)
+        assert (np.abs(f64(got) - want) <= step("bf16") * np.abs(want) + (1 + step("bf16")) * 2.0**-21 * size + smallest("bf16")).all()
+    for row, (page, slot) in {0: (0, 3), 2: (1, 3), 4: (3, 3)}.items():
+        want_k[1, page, slot], want_v[1, page, slot] = c.k[1, page, slot], v[row]
+    assert torch.equal(c.k, want_k) and torch.equal(c.v, want_v)
+
+
+@pytest.mark.parametrize("tree", [True, False])
+def test_a_run_of_a_pools_sequences_is_a_pool(tree):
+    """Sequences of different kinds in calls of their own (a prompt, single tokens): pool and row starts begin at the run's first sequence, rows keep
+    their numbers.  Together they are the one call's rows."""
+    counts, lengths = [1, 1, 180, 1], [300, 90, 40, 7]
+    c, q, start, bits = setup(counts, lengths, group=4, heads=2, dim=128, seed=21, tree=tree)
+    mask = None if bits is None else words(bits)
+    pool, starts = c.pool(), i32(start)
+    out, back = guarded(q)
+    for first, n in ((0, 2), (2, 1), (3, 1)):
+        view = c.pool()
+        view.sequences = n
+        view.table, view.length, view.held = pool.table + 4 * first * pool.table_stride, pool.length + 4 * first, pool.held + 4 * first
+        c.pool = lambda view=view: view
+        c.attend(q, out, starts[first:first + n + 1], mask)
+        torch.cuda.synchronize()
+        assert only(back, out, slice(0, start[first + n]))
+        del c.pool
+    use = bits
+    if bits is not None:
+        use = bits.copy()
+        for s, t in enumerate(counts):
+            use[start[s]:start[s + 1], t:] = False
+    want, bound = attention(f64(q), c.model, f64(c.k[0]), f64(c.v[0]), start, use, 0.125, c.dtype)
+    assert (np.abs(f64(out) - want) <= bound).all()
