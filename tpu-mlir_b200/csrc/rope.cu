@@ -4,9 +4,12 @@
 // formed and brought into one turn in 64 bits (at position 131072 a 32-bit product is off by 2^-8 of a radian), and its sine and cosine are
 // taken once for a (row, pair) and shared by all heads of the row through shared memory.
 //
-// What bounds it: HBM for prompts, where every element is read and written once (16 bytes a thread and access): 195 MB in 34.5 us, 5.65
-// TB/s, 0.86 of the measured rate.  For a token, launch and one row's chain sequence -> length -> page -> write (3.2 us).  Occupancy counts
-// for more than loads in flight a thread: four pieces a thread at once, at 64 registers, took 45 us.
+// What bounds it: HBM for prompts, where every element is read and written once (16 bytes a thread and access): 3 prompts of 1300 to 3900 tokens
+// appended, 195 MB, in 36.3 us, 5.4 TB/s, 0.82 of the measured copy rate; 8000 rows of 48 heads of 128 rotated alone, 197 MB, in 33.6 us,
+// 5.85 TB/s, 0.89.  For a token, launch and one row's chain sequence -> length -> page -> write (3.4 us).  Occupancy counts for more than loads in
+// flight a thread: four pieces a thread at once, at 64 registers, took 45 us for the prompts that took 37.
+// Not WIDE (half of the rotated part no multiple of 8 without interleaving, rows off 16 bytes): 2 bytes an access, in all of the head.  8000 rows of 64
+// heads of 96 with 24 rotated take 106 us where the bytes would take 30.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <math.h>
@@ -212,8 +215,8 @@ int launch_rope(RopeArgs& a, bool f16, bool wide, int sms, cudaStream_t s) {
   const int half = a.plan.rotary_dim / 2;
   wide = wide && a.plan.head_dim % 8 == 0 && (interleaved || half % 8 == 0);
   const int pieces = wide ? (interleaved ? a.plan.head_dim / 8 : half / 8 + (a.plan.head_dim - 2 * half) / 8) : a.plan.head_dim / 2;
-  // Rows of a block: three pieces a thread (8000 rows of 48 heads: 35 us with two rows, 37 with four, 41 with eight, 39 with one: sines are
-  // taken once for a row of a block, but short blocks hide each other's start), fewer where that leaves no four blocks an SM.  With still
+  // Rows of a block: three pieces a thread (8000 rows of 48 heads of 128: 33.5 us with two rows, 34.8 with four, 39.3 with eight, 36.8 with one:
+  // sines are taken once for a row of a block, but short blocks hide each other's start), fewer where that leaves no four blocks an SM.  With still
   // fewer rows the heads are spread over blocks until a thread has one piece, and every block takes the row's sines for itself.
   int rows = 1;
   while (rows < ROPE_ROWS && (int64_t)rows * a.heads * pieces < 3 * ROPE_THREADS) rows *= 2;

@@ -13,9 +13,11 @@
 // Two warps of a block only load, one keys and one values, with TMA boxes of as many rows as both a page and a unit are made of, ahead of
 // the products and across items, into a ring of stages of 64 keys and values; four warps compute.  Shared memory holds 64 elements
 // a row, swizzled by 16-byte pieces (piece ^ row % 8), so that ldmatrix meets no bank twice.  (Loading with 16-byte cp.async took 640
-// instructions a warp and unit: 108 us for 48 sequences of one token, 450 MB, that take 80 this way: 5.6 TB/s, 0.86 of the measured rate.)
+// instructions a warp and unit: 108 us for 48 sequences of one token, 450 MB, that take 81 this way: 5.55 TB/s, 0.85 of the measured rate.)
 //
-// What bounds it: DRAM; 10 us of a launch, the batch's lengths, the first unit's way through table and memory, and the join are fixed.
+// What bounds it: DRAM; 10 us of a launch, the batch's lengths, the first unit's way through table and memory, and the join are fixed.  At head size
+// 128 two blocks an SM fit up to 480 sequences (24 bytes of shared memory each); beyond, one does, and the grid of two an SM runs in two waves: one
+// token at 500 positions 5.2 TB/s for 470 sequences, 3.75 for 500, 4.0 for 1024.
 #include <math.h>
 
 #include "igemm.h"
@@ -508,18 +510,24 @@ int launch(const AttnArgs& a, int sms, cudaStream_t s) {
   return launch_join(a, blocks, S::ROWS, DIM, s);
 }
 
-// Rows of a tile by the batch's average of (node, head of the group) a cache head, which the host knows.  Both sides of each rule, bf16:
-//   up to 16 rows, 16-row tiles on mma.sync: 4 rows x 48 sequences of 200..8000 at dim 128 81.5 us (tcgen05 tiles 107.2), 4 rows x one of
-//     430 12.6 (32-row tiles 15.3, tcgen05 14.7), 16 rows x 16 sequences of 700..5000 41.7 (47.1), 8 rows x 64 of 20..600 29.4 (43.1);
-//   up to 32 rows, 32-row tiles: 24 x 16 sequences 43.1 (47.1), 32 x 16 45.0 (48.3), 32 x 64 short ones 37.7 (44.2), 20 rows x one of
-//     131,000 at dim 64 44.4 (45.0); from 48 rows on a 64-row tile of the same kernel was slower than tcgen05 (49 x 120,000, dim 64:
-//     55.2 against 43.2), and at dim 128 it spilled (96 rows x 16 sequences: 163 against 47), so there is none;
-//   more rows: tcgen05, 128 rows a tile, two streams of units a block.  Above 128 rows the two streams take two row tiles and share each
-//     unit's keys and values: 160 rows x 8 sequences of 700..8000 49.9 (two streams of one tile: 63.5), 512 rows 91.2 (124.5); below, one
-//     tile would idle: 96 rows 40.4 shared out by units against 44.5.
+// Rows of a tile by the average of (node, head of the group) a sequence of the call, which is what the host knows: rows / sequences * group.
+// Both sides of each rule, us, bf16, 32 heads on 8 of 128 unless said otherwise, contexts spread evenly over the range:
+//   up to 16 rows, 16-row tiles on mma.sync: 4 rows x 48 sequences of 200..8000 132.9 (32-row tiles 148.5, tcgen05 tiles 162.1), 4 rows x one of
+//     430 10.3 (10.7, 12.5), 16 rows x 16 of 700..5000 43.6 (44.5, 46.8), 8 rows x 64 of 20..600 30.8 (34.9, 44.5);
+//   up to 32 rows, 32-row tiles: 32 rows x 64 of 20..600 40.9 (16-row tiles 59.6, tcgen05 49.7), 20 rows x one of 131,000 at dim 64 71.9 (96.6,
+//     72.0), though 24 and 32 rows x 16 of 700..5000 49.5 and 49.9 (58.7 and 60.2; 47.3 and 47.7); from 48 rows on a 64-row tile of the same kernel was
+//     slower than tcgen05, and at dim 128 it spilled (96 rows x 16 sequences: 163 us), so there is none;
+//   more rows: tcgen05, 128 rows a tile, two streams of units a block (49 rows x one of 120,000 at dim 64 68.6, 32-row tiles 108.8; 96 rows x 16 52.3,
+//     110.1).  Above 128 rows the two streams take two row tiles and share each unit's keys and values: 160 rows x 8 of 700..8000 50.2 (two
+//     streams of one tile: 63.0), 512 rows 99.1 (129.0); below, one tile would idle: 96 rows 52.3 shared out by units against 58.9, 128 rows x 8 45.5
+//     against 49.3.
 // Chains of more than two row tiles on average (prompts) take the form in which tiles end at their own last node (a prompt of 4096 nodes
-// 158 us, without 491; in short calls its formula costs 1 us of 10).
-// Heads of more than 128 keep the 32-row tile: their scores and sums of two streams do not fit tensor memory beside one another.
+// 164 us, without 493; in short calls its formula costs 1 us of 10).
+// Sequences without rows, or of another kind, count in the average: 8 trees of 64 nodes at 12,500..16,000 positions take 130 us in a pool of 8 and 588 in one of
+// 64, a prompt of 4096 171 and 503, and 7425 in one of 1024.  A call over the run of sequences that has the rows is without that (130, 171).
+// Heads of more than 128 keep the 32-row tile: two streams' scores and sums do not fit tensor memory beside one another, and there is no form of
+// one stream, whose 256 columns of sums and twice 64 of scores would fit.  That is far from the floor where there are many rows: at 256, 8 trees of 64
+// nodes at 8000 positions take 2135 us (floor 81), a prompt of 2000 3141 (39), 48 tokens at 4000 278 (240).
 template <bool F16, int DIM>
 int launch_rows(const AttnArgs& a, int sms, cudaStream_t s) {
   const int64_t rows = (a.io.rows + a.pool.sequences - 1) / a.pool.sequences * a.group;

@@ -126,7 +126,7 @@ __device__ __forceinline__ uint64_t sees(const AttnArgs& a, int row, int node, i
 // ---- the line of units: which unit stands at a position of it
 // GROWS: for long chains (prompts).  Nodes of a chain do not see later ones, so its row tiles end at their own last node, rounded up to
 // what makes the line's sums a formula: the units of the committed positions, then `grow` for every tile, up to the sequence's end.
-// (A prompt of 4096 nodes, 32 heads on 8, 158 us instead of 491, eight of 1000 136 instead of 288.  Short items would lose 1 us of 10 to the
+// (A prompt of 4096 nodes, 32 heads on 8, 164 us instead of 493, eight of 1000 138 instead of 290.  Short items would lose 1 us of 10 to the
 // formula, so only calls of long chains have it.)
 template <bool GROWS>
 struct Line {
@@ -267,7 +267,7 @@ __device__ __forceinline__ long long lay_out(const AttnArgs& a, int tile_rows, i
 }
 
 // Positions of a block's run.  Short ones too: a short batch's units one after the other in a few blocks take longer than the join of many
-// parts (one token at 430 positions: 9.8 us with a unit a block, 11.2 with four; seven at 1000: 14.9 and 17.4).
+// parts (measured together: one token at 430 positions 9.8 us with a unit a block, 11.2 with four; seven at 1000 14.9 and 17.4).
 __device__ __forceinline__ long long run_of(long long total) {
   // (a 64-bit division takes hundreds of clocks)
   const long long all = total + gridDim.x - 1;

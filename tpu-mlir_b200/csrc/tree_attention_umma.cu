@@ -6,7 +6,7 @@
 //                 into tensor memory over the scores that they came from, rounded to the 16-bit type
 //   O += P V      128 x dim, P from tensor memory, V as it lies (positions x head: the operand is MN-major)
 // A block (one an SM: the rings of keys and values have to be deep, four to eight units, or their latency sets the pace: with two
-// stages and two blocks an SM 8 trees of 64 nodes over 16000 positions took 204 us where this takes 115) keeps two streams of this
+// stages and two blocks an SM 8 trees of 49 to 64 nodes over 9800 to 16,000 positions took 204 us where this took 115 in short runs) keeps two streams of this
 // going, each with four warps, two buffers of scores and sums of its own.  With more than 128 rows a cache head the streams are two row
 // tiles that share every unit of keys and values (PAIR); with fewer they take the units of one row tile in turn, and are merged at the
 // item's end.
@@ -14,8 +14,8 @@
 // weights up to 2^8 are as exact as those up to 1, and the division by the sum takes the base out again.
 //
 // What bounds it: DRAM up to 128 rows a cache head (a unit every 0.65 us an SM, 7.3 TB/s with what L2 holds, and 10 us of start and join; an
-// item more costs a block 5 us); beyond, exponentials, products and issue slots, 55, 55 and 46 % busy, wait for one another: 8 trees of 64
-// nodes, 256 rows, 428 MB and 95 GFLOP in 110 to 116 us, 830 TFLOP/s.
+// item more costs a block 5 us); beyond, exponentials, products and issue slots, 55, 55 and 46 % busy, wait for one another: 8 trees
+// of 49 to 64 nodes, up to 256 rows, 428 MB and 95 GFLOP in 135 us under steady load (707 TFLOP/s; the power cap's clocks) and 116 in short runs.
 #include <math.h>
 
 #include "igemm.h"
