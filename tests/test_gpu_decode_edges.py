@@ -1,5 +1,7 @@
 """What the decoding operators' contract says for inputs at its edge: values that are not finite in stages that are filled again, lengths and
 pages that the pool does not hold, scores past fp32's range, rows that no sequence names."""
+import threading
+
 import numpy as np
 import pytest
 
@@ -239,3 +241,55 @@ def test_a_run_of_a_pools_sequences_is_a_pool(tree):
             use[start[s]:start[s + 1], t:] = False
     want, bound = attention(f64(q), c.model, f64(c.k[0]), f64(c.v[0]), start, use, 0.125, c.dtype)
     assert (np.abs(f64(out) - want) <= bound).all()
+
+
+@pytest.mark.parametrize("counts,lengths,group,tree", [([3, 1, 7], [40, 100, 5], 2, True), ([40, 9, 0], [300, 20, 70], 4, True), ([200, 150], [20, 300], 4, False)])
+def test_rows_of_the_table_inside_wider_ones(counts, lengths, group, tree):
+    """A table_stride above table_width: every call stays within the rows.  And attention in place, chains whose tiles end at their last node too."""
+    c, q, start, bits = setup(counts, lengths, group=group, tree=tree, seed=3)
+    n, width = c.table.shape
+    wide = torch.full((n, width + 5), 77, dtype=torch.int32, device="cuda")
+    wide[:, :width] = c.table
+    c.table = wide[:, :width]
+    mask, out = None if bits is None else words(bits), torch.empty_like(q)
+    use = None if bits is None else bits.copy()
+    if use is not None:
+        for s, t in enumerate(counts):
+            use[start[s]:start[s + 1], t:] = False
+    want, bound = attention(f64(q), c.model, f64(c.k[0]), f64(c.v[0]), start, use, 0.125, c.dtype)
+    c.attend(q, out, i32(start), mask)
+    c.attend(q, q, i32(start), mask)
+    torch.cuda.synchronize()
+    assert torch.equal(q, out) and (np.abs(f64(out) - want) <= bound).all()
+    for call in (lambda x: x.fork([-1] + [0] * (n - 1)), lambda x: x.free([0] + [1] * (n - 1)), lambda x: x.reserve([30] * n)):
+        call(c)
+        call(c.model)
+        c.same_state()
+    assert c.status.item() == 0
+    assert bool((wide[:, width:] == 77).all())
+
+
+def test_calls_from_several_host_threads():
+    """A stream and a workspace each: the same results as one after the other."""
+    work = [setup([5 + s], [900], group=4, dim=128, seed=s) for s in range(4)]
+    alone, together = [torch.empty_like(q) for _, q, *_ in work], [torch.empty_like(q) for _, q, *_ in work]
+    held = [(i32(start), words(bits), c.workspace(q.shape[1]), torch.cuda.Stream()) for c, q, start, bits in work]
+    for (c, q, *_), o, (st, w, space, _) in zip(work, alone, held):
+        c.attend(q, o, st, w, space=space)
+    torch.cuda.synchronize()
+    failed = []
+
+    def run(i):
+        try:
+            (c, q, *_), (st, w, space, stream) = work[i], held[i]
+            for _ in range(100):
+                c.attend(q, together[i], st, w, stream=stream.cuda_stream, space=space)
+            stream.synchronize()
+        except Exception as e:
+            failed.append(e)
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed and all(torch.equal(a, b) for a, b in zip(alone, together))
